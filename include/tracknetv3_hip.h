@@ -563,6 +563,31 @@ int tnv3_median_u8(const unsigned char* frames, unsigned char* median, uint16_t*
 int tnv3_absdiff_sum_u8(const unsigned char* frames, const uint16_t* median_x2, unsigned char* out, int frames_n,
                         long pixels, tnv3_stream_t stream);
 
+/* ---- position-wise layers --------------------------------------------------------------------------------
+ * The reference's own layers of this kind are the 1x1 head and InpaintNet's Conv1d + activation (model.py:45, 76-87); these are their general
+ * form over rows of any width, and the gated block built from them.  dtype: 0 fp32, 1 bf16, 2 fp16, of EVERY tensor of a call; sums are fp32.
+ * act: 0 none, 1 leaky ReLU (0.01), 2 sigmoid, 3 ReLU, 4 SiLU (z sigmoid z), 5 GELU (z Phi(z)), 6 GELU in its tanh form.
+ *   linear   z = x w^T + bias, y = act(z) + residual       x (rows, k), w (n, k), bias (n) or NULL, residual (rows, n) or NULL, y (rows, n)
+ *   gated    [g | u] = x w^T + bias, h = act(g) * u        w (2 n, k): the gate's n rows, then the other factor's; bias (2 n) or NULL, h (rows, n)
+ * pre (may be NULL): the pre-activation z, (rows, n) / (rows, 2 n), that the backward call takes (linear with act 0 needs none).  Tensors are
+ * contiguous; bases and widths may have any alignment (16-byte aligned ones are faster).  1 <= rows <= 2^30, 1 <= widths <= 2^20.  An output must
+ * not overlap an input.  Same inputs, same bits.  The workspace (16-byte aligned, at least the queried size; the query may be 0) is scratch for
+ * the one call. */
+size_t tnv3_linear_forward_workspace_bytes(long rows, int k, int n, int dtype);
+int tnv3_linear_forward(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre, void* workspace,
+                        size_t workspace_bytes, long rows, int k, int n, int act, int dtype, tnv3_stream_t stream);
+/* dz = dy act'(pre); dx = dz w, dw = dz^T x, db = column sums of dz (each may be NULL: not wanted).  The residual's gradient is dy. */
+size_t tnv3_linear_backward_workspace_bytes(long rows, int k, int n, int act, int dtype);
+int tnv3_linear_backward(const void* dy, const void* x, const void* w, const void* pre, void* dx, void* dw, void* db, void* workspace,
+                         size_t workspace_bytes, long rows, int k, int n, int act, int dtype, tnv3_stream_t stream);
+size_t tnv3_gated_linear_forward_workspace_bytes(long rows, int k, int n, int dtype);
+int tnv3_gated_linear_forward(const void* x, const void* w, const void* bias, void* h, void* pre, void* workspace, size_t workspace_bytes,
+                              long rows, int k, int n, int act, int dtype, tnv3_stream_t stream);
+/* dz = [dh u act'(g) | dh act(g)] (rows, 2 n); dx (rows, k), dw (2 n, k), db (2 n) from it as above. */
+size_t tnv3_gated_linear_backward_workspace_bytes(long rows, int k, int n, int act, int dtype);
+int tnv3_gated_linear_backward(const void* dh, const void* x, const void* w, const void* pre, void* dx, void* dw, void* db, void* workspace,
+                               size_t workspace_bytes, long rows, int k, int n, int act, int dtype, tnv3_stream_t stream);
+
 /* Diagnostics (the register-only MFMA probe, timing twins with deliberately wrong results) are NOT part of this library:
  * they are built from the same sources into libtnv3_diag.so, declared in include/tracknetv3_hip_diag.h. */
 

@@ -319,6 +319,79 @@ inline emu_f32x4 __builtin_amdgcn_mfma_f32_16x16x4f32(float a, float b, emu_f32x
   return d;
 }
 
+// ---- 16-bit operands (kernels/linear_*.h): conversions, the 32x32x16 / 16x16x32 fragments, the transposing LDS read
+inline float emu_bf16_up(unsigned short h) { unsigned u = (unsigned)h << 16; float f; memcpy(&f, &u, 4); return f; }
+inline unsigned short emu_bf16_dn(float f) {                 // round to nearest even, NaN kept
+  unsigned u; memcpy(&u, &f, 4);
+  if ((u & 0x7fffffffu) > 0x7f800000u) return (unsigned short)((u >> 16) | 0x40u);
+  return (unsigned short)((u + 0x7fffu + ((u >> 16) & 1u)) >> 16);
+}
+inline float emu_f16_up(unsigned short h) {
+  const int e = (h >> 10) & 31, m = h & 1023;
+  float f = e == 31 ? (m ? NAN : INFINITY) : (e ? ldexpf((float)(1024 + m), e - 25) : ldexpf((float)m, -24));
+  return h & 0x8000 ? -f : f;
+}
+inline unsigned short emu_f16_dn(float f) {                  // round to nearest even
+  unsigned u; memcpy(&u, &f, 4);
+  const unsigned short sign = (unsigned short)((u >> 16) & 0x8000u);
+  const float a = fabsf(f);
+  if (f != f) return (unsigned short)(sign | 0x7e00u);
+  if (a >= 65520.0f) return (unsigned short)(sign | 0x7c00u);
+  if (a < 6.103515625e-5f) return (unsigned short)(sign | (unsigned short)lrintf(ldexpf(a, 24)));     // subnormal (or the least normal)
+  int e; const float m = frexpf(a, &e);                      // a = m 2^e, 0.5 <= m < 1
+  return (unsigned short)(sign | (unsigned)(((e + 14) << 10) + (long)lrintf(ldexpf(m, 11)) - 1024));
+}
+typedef short emu_s8 __attribute__((ext_vector_type(8)));
+typedef short emu_s4 __attribute__((ext_vector_type(4)));
+namespace emu { inline emu_s8& frag(unsigned wave, int operand, unsigned lane) { static emu_s8 buf[MAX_WAVES][2][WAVE]; return buf[wave][operand][lane]; } }
+// A[l & 31][8 (l >> 5) + 0..7], B likewise; D as for 32x32x2.  The sum of the 16 products is taken in fp64 and rounded once into the accumulator.
+inline emu_f32x16 emu_mfma_32x32x16(emu_s8 a, emu_s8 b, emu_f32x16 c, float (*up)(unsigned short)) {
+  emu::State& s = emu::S(); const unsigned w = emu::wave_id(), l = emu::lane_id();
+  if (s.wave_size[w] != 64) { fprintf(stderr, "emu: MFMA needs a full wave\n"); abort(); }
+  emu::frag(w, 0, l) = a; emu::frag(w, 1, l) = b;
+  emu::wave_barrier();
+  emu_f32x16 d;
+  double bv[16];
+  for (unsigned k = 0; k < 16; ++k) bv[k] = up((unsigned short)emu::frag(w, 1, (l & 31) + 32 * (k >> 3))[k & 7]);
+  for (int r = 0; r < 16; ++r) {
+    const unsigned row = (r & 3) + 8 * (r >> 2) + 4 * (l >> 5);
+    double acc = c[r];
+    for (unsigned k = 0; k < 16; ++k) acc += (double)up((unsigned short)emu::frag(w, 0, row + 32 * (k >> 3))[k & 7]) * bv[k];
+    d[r] = (float)acc;
+  }
+  emu::wave_barrier();
+  return d;
+}
+// A[l & 15][8 (l >> 4) + 0..7], B likewise; D register r -> row 4 (l >> 4) + r, column l & 15
+inline emu_f32x4 emu_mfma_16x16x32(emu_s8 a, emu_s8 b, emu_f32x4 c, float (*up)(unsigned short)) {
+  emu::State& s = emu::S(); const unsigned w = emu::wave_id(), l = emu::lane_id();
+  if (s.wave_size[w] != 64) { fprintf(stderr, "emu: MFMA needs a full wave\n"); abort(); }
+  emu::frag(w, 0, l) = a; emu::frag(w, 1, l) = b;
+  emu::wave_barrier();
+  emu_f32x4 d;
+  for (int r = 0; r < 4; ++r) {
+    const unsigned row = 4 * (l >> 4) + r;
+    double acc = c[r];
+    for (unsigned k = 0; k < 32; ++k)
+      acc += (double)up((unsigned short)emu::frag(w, 0, row + 16 * (k >> 3))[k & 7]) * (double)up((unsigned short)emu::frag(w, 1, (l & 15) + 16 * (k >> 3))[k & 7]);
+    d[r] = (float)acc;
+  }
+  emu::wave_barrier();
+  return d;
+}
+// ds_read_b64_tr_b16: in each group of 16 lanes, lane q's address names 4 elements of row q >> 2 (columns 4 (q & 3) ..); lane q gets column q of
+// the four rows
+inline emu_s4 emu_lds_tr4(const unsigned short* p) {
+  emu::State& s = emu::S(); const unsigned w = emu::wave_id(), l = emu::lane_id();
+  uint64_t v; memcpy(&v, p, 8);
+  s.xchg[w][3][l] = v;
+  emu::wave_barrier();
+  emu_s4 d;
+  for (int j = 0; j < 4; ++j) d[j] = (short)(s.xchg[w][3][(l & ~15u) + 4 * j + ((l & 15) >> 2)] >> (16 * (l & 3)));
+  emu::wave_barrier();
+  return d;
+}
+
 // LDS DMA: LDS[base + lane*size] <- *gsrc (per-lane source, wave-uniform LDS base = lane 0's argument)
 inline void __builtin_amdgcn_global_load_lds(const __attribute__((address_space(1))) void* g, __attribute__((address_space(3))) void* l,
                                              unsigned size, int offset, unsigned) {

@@ -1,0 +1,159 @@
+"""Shared by the CPU (emulator) and GPU tests of the position-wise layers: 64-bit oracles, element-wise error bounds derived from the types, and the
+exact integer cases (operands in {-1, 0, 1} whose sums every type holds exactly: any wrong, missing or doubled index shows)."""
+import torch
+import torch.nn.functional as F
+
+ACTS = ("none", "leaky_relu", "sigmoid", "relu", "silu", "gelu", "gelu_tanh")
+DTYPES = (torch.float32, torch.bfloat16, torch.float16)
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 2.0 ** -126, torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -24}      # below: absolute instead of relative rounding
+LARGEST_EXACT = {torch.float32: 1 << 24, torch.bfloat16: 1 << 8, torch.float16: 1 << 11}
+
+
+def act64(z, act):
+    return {"none": lambda t: t, "leaky_relu": lambda t: F.leaky_relu(t, 0.01), "sigmoid": torch.sigmoid, "relu": F.relu, "silu": F.silu, "gelu": F.gelu,
+            "gelu_tanh": lambda t: F.gelu(t, approximate="tanh")}[act](z)
+
+
+def oracle(x, w, b=None, r=None, act="none", gated=False, dy=None):
+    """{y, z[, dz, x, w, b, r gradients]} in float64 on the CPU."""
+    d = {k: t.detach().cpu().double().requires_grad_() for k, t in (("x", x), ("w", w), ("b", b), ("r", r)) if t is not None}
+    z = F.linear(d["x"], d["w"], d.get("b"))
+    z.retain_grad()
+    if gated:
+        g, u = z.chunk(2, -1)
+        y = act64(g, act) * u
+    else:
+        y = act64(z, act)
+        y = y + d["r"] if "r" in d else y
+    out = {"y": y.detach(), "z": z.detach()}
+    if dy is not None:
+        y.backward(dy.cpu().double())
+        out["dz"] = z.grad
+        out.update({"d" + k: t.grad for k, t in d.items()})
+    return out
+
+
+# |act''| <= 1.2 and |act'| <= 1.13 for every activation of ACTS away from the kinks of relu / leaky_relu
+L1, L2 = 1.13, 1.2
+
+
+def bounds(x, w, b, r, act, gated, dy, dtype):
+    """Largest allowed |error| per element of y and the gradients, from: inputs exact; sums in fp32 (a chain of at most 6 / 16 roundings per term
+    of the contraction plus 64, and 2^-23 per term left out of the fp32 split); the activation within 2^-18 of its scale; one rounding of
+    z, dz and each output to the type."""
+    u, tiny = HALF_STEP[dtype], TINY[dtype]
+    o = oracle(x, w, b, r, act, gated, dy)
+    x64, w64 = x.detach().cpu().double().abs(), w.detach().cpu().double().abs()
+    x2 = x64.reshape(-1, x64.shape[-1])
+
+    def chain(terms):
+        return (6 * terms / 16 + 64) * 2.0 ** -24 + 2.0 ** -23
+
+    e_act = 2.0 ** -18 if dtype != torch.float32 else 2.0 ** -21
+    z = o["z"].abs().reshape(-1, w64.shape[0])
+    ez = chain(x2.shape[1]) * (x2 @ w64.t() + (0 if b is None else b.detach().cpu().double().abs()))          # of the fp32 sum
+    y = o["y"].abs().reshape(z.shape[0], -1)
+    out = {}
+    if gated:
+        g, uu = z.chunk(2, -1)
+        eg, eu = ez.chunk(2, -1)
+        a = g + 1
+        out["y"] = u * y + tiny + (L1 * eg + e_act * a) * (uu + eu) + a * eu
+    else:
+        rr = 0 if r is None else r.detach().cpu().double().abs().reshape(y.shape)
+        out["y"] = u * y + tiny + L1 * ez + e_act * (z + 1) + 2.0 ** -23 * (z + rr)
+    if dy is None:
+        return out
+    d = dy.cpu().double().abs().reshape(y.shape)
+    ezs = ez + u * z + tiny                                  # of the pre-activation as it is kept
+    if gated:
+        g, uu = z.chunk(2, -1)
+        eg, eu = ezs.chunk(2, -1)
+        edz = torch.cat([d * (L1 * eu + (L2 * eg + e_act * (g + 1)) * (uu + eu)), d * (L1 * eg + e_act * (g + 1))], -1)
+        act_pass = True
+    else:
+        act_pass = act != "none"
+        edz = d * (L2 * ezs + e_act * (z + 1)) if act_pass else torch.zeros_like(z)
+    dz = o["dz"].abs().reshape(z.shape)
+    edb = edz + 2.0 ** -23 * dz
+    if act_pass:
+        edz = edz + (u + 2.0 ** -23) * dz + tiny
+    rows = z.shape[0]
+    out["dx"] = (edz + chain(z.shape[1]) * (dz + edz)) @ w64 + u * o["dx"].abs().reshape(x2.shape) + tiny
+    out["dw"] = (edz + chain(rows) * (dz + edz)).t() @ x2 + u * o["dw"].abs() + tiny
+    if b is not None:
+        out["db"] = (edb + chain(rows) * (dz + edb)).sum(0) + u * o["db"].abs() + tiny
+    return out
+
+
+def make(rows, k, n, dtype, gated=False, bias=True, residual=False, seed=0, device="cpu", scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    wide = 2 * n if gated else n
+    x = (torch.randn(rows, k, generator=g) * scale).to(dtype).to(device)
+    w = (torch.randn(wide, k, generator=g) / k ** 0.5).to(dtype).to(device)
+    b = torch.randn(wide, generator=g).to(dtype).to(device) if bias else None
+    r = torch.randn(rows, n, generator=g).to(dtype).to(device) if residual else None
+    dy = torch.randn(rows, n, generator=g).to(dtype).to(device)
+    return x, w, b, r, dy
+
+
+def run(x, w, b, r, act, gated, dy):
+    """The framework's forward and backward: {y, dx, dw[, db, dr]}."""
+    from tracknetv3_amd import feedforward as ff
+    leaves = {k: t.detach().requires_grad_() for k, t in (("x", x), ("w", w), ("b", b), ("r", r)) if t is not None}
+    if gated:
+        y = ff.gated_linear(leaves["x"], leaves["w"], leaves.get("b"), act=act)
+    else:
+        y = ff.linear(leaves["x"], leaves["w"], leaves.get("b"), residual=leaves.get("r"), act=act)
+    grads = torch.autograd.grad(y, list(leaves.values()), dy)
+    return {"y": y.detach(), **{"d" + k: g for k, g in zip(leaves, grads)}}
+
+
+def check_close(rows, k, n, dtype, act, gated, bias, residual, device, seed=0):
+    x, w, b, r, dy = make(rows, k, n, dtype, gated, bias, residual, seed, device)
+    got = run(x, w, b, r, act, gated, dy)
+    if act in ("relu", "leaky_relu"):
+        # away from the kink: a sum within its own error of 0 has no determined derivative
+        z = oracle(x, w, b, r, act, gated)["z"]
+        z = z.chunk(2, -1)[0] if gated else z
+        assert (z.abs() > 1e-6).all()
+    want, tol = oracle(x, w, b, r, act, gated, dy), bounds(x, w, b, r, act, gated, dy, dtype)
+    for name, limit in tol.items():
+        err = (got[name].cpu().double() - want[name]).abs().reshape(limit.shape)
+        assert torch.isfinite(got[name]).all(), name
+        worst = (err / limit).max().item()
+        assert worst <= 1.0, (name, worst, err.max().item())
+    if r is not None:
+        assert torch.equal(got["dr"], dy)
+
+
+def sparse_signs(shape, density, gen):
+    return torch.randint(0, 2, shape, generator=gen) * 2.0 - 1.0 if density >= 1 else \
+        (torch.rand(shape, generator=gen) < density).float() * (torch.randint(0, 2, shape, generator=gen) * 2.0 - 1.0)
+
+
+def check_exact(rows, k, n, dtype, gated, bias, residual, device, act="relu", seed=0):
+    """Integer operands: every sum, product and rounding is exact, so the results are equal to the oracle's.  Densities keep the sums far below the
+    largest integer up to which the type holds all."""
+    g = torch.Generator().manual_seed(seed)
+    wide = 2 * n if gated else n
+
+    def density(terms):                   # about 12 nonzero products at most, each of size 1
+        return min(1.0, (12.0 / terms) ** 0.5)
+
+    # two factors of a product share the density of its length; the longest contraction decides
+    p = density(max(rows, k, wide))
+    x = sparse_signs((rows, k), max(p, density(k)), g)
+    w = sparse_signs((wide, k), max(p, density(k)), g)
+    dy = sparse_signs((rows, n), min(p, density(max(rows, wide))), g)
+    b = torch.randint(-2, 3, (wide,), generator=g).float() if bias else None
+    r = torch.randint(-2, 3, (rows, n), generator=g).float() if residual else None
+    act = "none" if act == "none" else "relu"
+    want = oracle(x, w, b, r, act, gated, dy)
+    lim = LARGEST_EXACT[dtype]
+    assert all(v.abs().max() <= lim for v in want.values()), {q: v.abs().max().item() for q, v in want.items()}
+    cast = [None if t is None else t.to(dtype).to(device) for t in (x, w, b, r, dy)]
+    got = run(*cast[:4], act, gated, cast[4])
+    for name, v in got.items():
+        assert torch.equal(v.cpu().double(), want[name]), (name, (v.cpu().double() != want[name]).nonzero()[:4].tolist())

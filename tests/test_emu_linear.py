@@ -1,0 +1,159 @@
+"""CPU: the position-wise layers (linear, gated_linear and their backward passes) on the host SIMT emulator -- index arithmetic, tails and write-out
+of the unchanged kernels -- and the refusals of their entry points."""
+import ctypes
+
+import pytest
+import torch
+
+import linear_common as lc
+from tracknetv3_amd import _lib, feedforward as ff, ops
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 64, 32), (3, 5, 7), (17, 72, 40), (33, 129, 65), (130, 40, 136)])
+def test_exact_integers(emu, rows, k, n, gated, dtype):
+    lc.check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device="cpu", seed=rows + k)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated,act", [(False, a) for a in lc.ACTS] + [(True, a) for a in lc.ACTS if a != "none"])
+def test_activations_and_gradients(emu, act, gated, dtype):
+    lc.check_close(9, 40, 24, dtype, act, gated, bias=True, residual=not gated, device="cpu", seed=3)
+
+
+def test_no_bias_no_residual_and_leading_shape(emu):
+    x = torch.randn(2, 3, 16)
+    w = torch.randn(8, 16) / 4
+    y = ff.linear(x, w)
+    assert y.shape == (2, 3, 8) and torch.allclose(y, x @ w.t(), atol=1e-6)
+    h = ff.gated_linear(x.transpose(0, 1), w)                     # not contiguous: copied by the differentiable entry
+    assert h.shape == (3, 2, 4)
+
+
+def test_split_contraction_joins_all_parts(emu, monkeypatch):
+    """Few rows and a long contraction: the parts' partial sums are joined."""
+    lib = _lib.load()
+    assert lib.tnv3_linear_forward_workspace_bytes(40, 1100, 24, 0) > 0
+    for dtype in lc.DTYPES:
+        lc.check_exact(40, 1100, 24, dtype, False, True, True, "cpu")
+        lc.check_exact(40, 1100, 24, dtype, True, True, False, "cpu")
+
+
+def test_fp32_keeps_infinities_and_nan_where_they_belong(emu):
+    inf, nan = float("inf"), float("nan")
+    x = torch.randn(5, 40)
+    w = torch.randn(6, 40)
+    x[1, 3], x[2, 7], x[3, 2], x[4, 0] = inf, -inf, nan, 3.4e38       # 3.4e38: beyond bf16's largest, finite in fp32
+    w[:, 0] = torch.tensor([0.25, -0.25, 0.5, -0.5, 0.125, 0.0])
+    w[5, 3] = 0.0                                                     # inf * 0 = NaN
+    y = ff.linear(x, w)
+    want = (x.double() @ w.double().t()).float()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    ok = torch.isfinite(want)
+    assert torch.allclose(y[ok], want[ok], rtol=1e-5, atol=1e-5)
+    assert torch.equal(torch.sign(y[torch.isinf(want)]), torch.sign(want[torch.isinf(want)]))
+
+
+def test_zero_rows(emu):
+    x = torch.zeros(0, 12, requires_grad=True)
+    w = torch.randn(10, 12, requires_grad=True)
+    b = torch.randn(10, requires_grad=True)
+    for y in (ff.linear(x, w, b, act="gelu"), ff.gated_linear(x, w, b)):
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.zeros_like(y))
+        assert dx.shape == (0, 12) and not dw.any() and not db.any()
+
+
+def test_only_the_gradients_that_are_wanted(emu):
+    x, w, b, r, dy = lc.make(6, 24, 16, torch.float32, residual=True)
+    w.requires_grad_()
+    y = ff.linear(x, w, b, r, act="silu")
+    (dw,) = torch.autograd.grad(y, (w,), dy)
+    want = lc.oracle(x, w, b, r, "silu", False, dy)["dw"]
+    assert torch.allclose(dw.double(), want, atol=1e-5)
+    r.requires_grad_()
+    y = ff.linear(x, w.detach(), b, r)
+    (dr,) = torch.autograd.grad(y, (r,), dy)
+    assert torch.equal(dr, dy)
+
+
+def test_gradients_against_differences(emu):
+    """Central differences of sum(y * dy) along random directions; fp32 forward, step 2^-7: the difference's own error is about
+    (step^2 |third derivative| + 2^-24 |value| / step) -- 1e-3 of the gradient's scale."""
+    for gated in (False, True):
+        x, w, b, _, dy = lc.make(7, 20, 12, torch.float32, gated)
+        got = lc.run(x, w, b, None, "gelu", gated, dy)
+        gen = torch.Generator().manual_seed(9)
+        for name, t in (("dx", x), ("dw", w), ("db", b)):
+            v = torch.randn(t.shape, generator=gen)
+            h = 2.0 ** -7
+
+            def f(s):
+                a = {"dx": x, "dw": w, "db": b}
+                a[name] = t + s * v
+                y = ff.gated_linear(a["dx"], a["dw"], a["db"], act="gelu") if gated else ff.linear(a["dx"], a["dw"], a["db"], act="gelu")
+                return (y.double() * dy.double()).sum()
+            num, ana = ((f(h) - f(-h)) / (2 * h)).item(), (got[name].double() * v.double()).sum().item()
+            assert abs(num - ana) <= 3e-3 * (got[name].double().norm() * v.double().norm()).item(), (gated, name, num, ana)
+
+
+def test_block_runs_as_a_model_uses_it(emu):
+    torch.manual_seed(1)
+    block = ff.GatedFeedForward(24, 40, bias=True)
+    assert list(block.state_dict()) == ["weight", "weight_out", "bias", "bias_out"]
+    x = torch.randn(3, 5, 24, requires_grad=True)
+    y = block(x)
+    y.square().mean().backward()
+    p = {k: v.detach().double().requires_grad_() for k, v in block.named_parameters()}
+    x64 = x.detach().double().requires_grad_()
+    g, u = torch.nn.functional.linear(x64, p["weight"], p["bias"]).chunk(2, -1)
+    ref = torch.nn.functional.linear(torch.nn.functional.silu(g) * u, p["weight_out"], p["bias_out"]) + x64
+    ref.square().mean().backward()
+    assert torch.allclose(y.double(), ref, atol=1e-5)
+    for got, want in [(x.grad, x64.grad)] + [(q.grad, p[k].grad) for k, q in block.named_parameters()]:
+        assert torch.allclose(got.double(), want, rtol=1e-4, atol=1e-6)
+    lin = ff.Linear(24, 8, act="relu")
+    assert list(lin.state_dict()) == ["weight", "bias"] and torch.allclose(lin(x), torch.relu(torch.nn.functional.linear(x, lin.weight, lin.bias)), atol=1e-5)
+
+
+def test_refusals(emu):
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    err = _lib.Tnv3Error
+    for call, text in ((lambda: ops.linear(x.double(), w.double()), "float32, bfloat16 or float16"),
+                       (lambda: ops.linear(x, w.bfloat16()), "must be"),
+                       (lambda: ops.linear(x, torch.zeros(6, 9)), "does not match"),
+                       (lambda: ops.linear(x, w, torch.zeros(5)), "bias"),
+                       (lambda: ops.linear(x, w, None, torch.zeros(4, 1)), "residual"),
+                       (lambda: ops.linear(x, w, act=7), "unknown activation"),
+                       (lambda: ops.linear(x.t().contiguous().t(), w), "contiguous"),
+                       (lambda: ops.gated_linear(x, torch.zeros(5, 8)), "even number"),
+                       (lambda: ops.gated_linear(torch.zeros(4, 0), torch.zeros(6, 0)), "bad weight"),
+                       (lambda: ops.linear_backward(torch.zeros(4, 6), x, w, None, ops.ACT_SILU), "pre-activation"),
+                       (lambda: ops.gated_linear_backward(torch.zeros(4, 3), x, w, None), "pre-activation"),
+                       (lambda: ops.linear_backward(torch.zeros(4, 5), x, w), "upstream"),
+                       (lambda: ops.gated_linear_backward(torch.zeros(4, 3), x, w, torch.zeros(4, 3)), "pre")):
+        with pytest.raises(err, match=text):
+            call()
+    with pytest.raises(ValueError, match="unknown activation"):
+        ff.linear(x, w, act="tanh")
+    with pytest.raises(ValueError, match="expects"):
+        ff.GatedFeedForward(8, 4)(torch.zeros(2, 7))
+    # the C entries themselves
+    lib = _lib.load()
+    p, null = _lib.ptr, ctypes.c_void_p(0)
+    y = torch.zeros(4, 6)
+
+    def fwd(rows=4, k=8, n=6, act=0, dtype=0, xp=None, ws=null, nws=0):
+        return lib.tnv3_linear_forward(p(x) if xp is None else xp, p(w), null, null, p(y), null, ws, nws, rows, k, n, act, dtype, null)
+    assert fwd() == 0
+    for bad in (dict(rows=0), dict(k=0), dict(n=-1), dict(rows=(1 << 30) + 1), dict(k=(1 << 20) + 1), dict(n=(1 << 20) + 1), dict(act=7), dict(act=-1),
+                dict(dtype=3), dict(xp=null)):
+        assert fwd(**bad) != 0, bad
+    assert lib.tnv3_linear_backward(p(y), p(x), p(w), null, p(x), null, null, null, 0, 4, 8, 6, 0, 0, null) != 0           # no workspace
+    long_k = lib.tnv3_linear_forward_workspace_bytes(40, 1100, 24, 0)
+    big = [torch.zeros(s) for s in ((40, 1100), (24, 1100), (40, 24))]
+    ws = torch.zeros(long_k // 4)
+    args = [p(big[0]), p(big[1]), null, null, p(big[2]), null]
+    assert lib.tnv3_linear_forward(*args, p(ws), long_k - 4, 40, 1100, 24, 0, 0, null) != 0                                  # too small
+    assert lib.tnv3_linear_forward(*args, p(ws), long_k, 40, 1100, 24, 0, 0, null) == 0
+    assert lib.tnv3_linear_forward_workspace_bytes(0, 1, 1, 0) == 0

@@ -1,0 +1,190 @@
+"""GPU: the position-wise layers on the MI355X through the public entry points -- every kernel variant's sizes, alignments, streams, graph replay."""
+import pytest
+import torch
+
+import linear_common as lc
+from tracknetv3_amd import feedforward as ff, ops
+
+pytestmark = pytest.mark.gpu
+
+# one row, a few, the border of the few-rows kernels, ragged tiles, whole tiles, long contractions with few tiles, many tiles
+SHAPES = [(1, 1, 1), (1, 64, 32), (1, 2048, 512), (2, 40, 24), (13, 1003, 137), (16, 256, 256), (17, 72, 40), (31, 130, 66), (33, 512, 200), (64, 1000, 264),
+          (65, 33, 1030), (128, 128, 128), (130, 40, 136), (200, 4096, 96), (257, 264, 520), (300, 1001, 333), (512, 384, 128), (1000, 600, 1000),
+          (2048, 512, 768), (4099, 72, 136), (3000, 2000, 1504)]
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_exact_integers(gpu_device, rows, k, n, gated, dtype):
+    lc.check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device=gpu_device, seed=rows + k)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated,act", [(False, a) for a in lc.ACTS] + [(True, a) for a in lc.ACTS if a != "none"])
+@pytest.mark.parametrize("rows,k,n", [(1, 96, 40), (9, 40, 24), (150, 264, 136)])
+def test_activations_and_gradients(gpu_device, rows, k, n, act, gated, dtype):
+    lc.check_close(rows, k, n, dtype, act, gated, bias=True, residual=not gated, device=gpu_device, seed=3)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+def test_large_against_64_bits(gpu_device, gated, dtype):
+    lc.check_close(1027, 776, 1048, dtype, "silu" if gated else "gelu", gated, bias=True, residual=not gated, device=gpu_device, seed=5)
+    lc.check_close(520, 1031, 517, dtype, "sigmoid", gated, bias=False, residual=False, device=gpu_device, seed=6)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("rows", [1, 40, 300])
+def test_views_whose_base_is_not_aligned(gpu_device, rows, dtype):
+    """Contiguous tensors that start one element into their storage."""
+    k, n = 264, 136
+
+    def shifted(t):
+        s = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)[1:]
+        s.copy_(t.reshape(-1))
+        return s.view(t.shape)
+    for gated in (False, True):
+        x, w, b, r, dy = lc.make(rows, k, n, dtype, gated, True, not gated, 2, gpu_device)
+        want = lc.run(x, w, b, r, "silu", gated, dy)
+        got = lc.run(shifted(x), shifted(w), shifted(b), None if r is None else shifted(r), "silu", gated, shifted(dy))
+        tol = lc.bounds(x, w, b, r, "silu", gated, dy, dtype)
+        for name, limit in tol.items():
+            assert ((got[name] - want[name]).cpu().double().abs().reshape(limit.shape) <= 2 * limit).all(), name
+
+
+def test_fp32_keeps_infinities_and_nan_where_they_belong(gpu_device):
+    inf, nan = float("inf"), float("nan")
+    for rows in (5, 200):
+        x, w = torch.randn(rows, 40), torch.randn(66, 40)
+        x[1, 3], x[2, 7], x[3, 2], x[4, 0] = inf, -inf, nan, 3.4e38
+        w[:, 0] = torch.randn(66).sign() * 0.25
+        w[5, 3] = 0.0
+        y = ff.linear(x.to(gpu_device), w.to(gpu_device)).cpu()
+        want = (x.double() @ w.double().t()).float()
+        assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+        ok = torch.isfinite(want)
+        assert torch.allclose(y[ok], want[ok], rtol=1e-5, atol=1e-4)
+        assert torch.equal(torch.sign(y[torch.isinf(want)]), torch.sign(want[torch.isinf(want)]))
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+def test_rows_behind_the_last_stay_as_they_were(gpu_device, dtype):
+    """Outputs are written up to their last element and not beyond, at sizes that end inside a tile, a vector and a row block."""
+    lib, p = ops._lib.load(), ops._lib.ptr
+    code = ops._LINEAR_DTYPES[dtype]
+    for rows, k, n in ((1, 40, 24), (5, 33, 17), (37, 136, 72), (130, 72, 140)):
+        x, w, _, _, dy = lc.make(rows, k, n, dtype, device=gpu_device)
+        outs = {name: torch.full((size + 64,), 7.0, dtype=dtype, device=gpu_device) for name, size in
+                (("y", rows * n), ("pre", rows * n), ("dx", rows * k), ("dw", n * k), ("db", n))}
+        s = ops._lib.stream_ptr(x)
+        nf, nb = lib.tnv3_linear_forward_workspace_bytes(rows, k, n, code), lib.tnv3_linear_backward_workspace_bytes(rows, k, n, 4, code)
+        guard = 4096
+        ws = torch.full((max(nf, nb) + guard,), 85, dtype=torch.uint8, device=gpu_device)
+        assert lib.tnv3_linear_forward(p(x), p(w), None, None, p(outs["y"]), p(outs["pre"]), p(ws), nf, rows, k, n, 4, code, s) == 0
+        assert lib.tnv3_linear_backward(p(dy), p(x), p(w), p(outs["pre"]), p(outs["dx"]), p(outs["dw"]), p(outs["db"]), p(ws), nb, rows, k, n, 4, code, s) == 0
+        for name, t in outs.items():
+            assert (t[-64:] == 7).all() and torch.isfinite(t).all(), (name, rows)
+        assert (ws[-guard:] == 85).all()
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+def test_same_bits_from_run_to_run_and_on_another_stream(gpu_device, dtype):
+    side = torch.cuda.Stream(gpu_device)
+    for rows, k, n in ((1, 1024, 512), (48, 2048, 256), (700, 512, 640)):
+        x, w, b, _, dy = lc.make(rows, k, n, dtype, True, device=gpu_device)
+        first = lc.run(x, w, b, None, "silu", True, dy)
+        again = lc.run(x, w, b, None, "silu", True, dy)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            other = lc.run(x, w, b, None, "silu", True, dy)
+        torch.cuda.current_stream().wait_stream(side)
+        for name in first:
+            assert torch.equal(first[name], again[name]) and torch.equal(first[name], other[name]), name
+
+
+@pytest.mark.parametrize("rows", [1, 24, 400])
+def test_block_captured_and_replayed(gpu_device, rows):
+    """The whole block, forward and backward, in one graph: replays on new inputs equal the eager results, with eager work in between."""
+    torch.manual_seed(0)
+    block = ff.GatedFeedForward(256, 640, bias=True).to(gpu_device, torch.bfloat16)
+    params = list(block.parameters())
+    x = torch.randn(rows, 256, device=gpu_device, dtype=torch.bfloat16, requires_grad=True)
+    dy = torch.randn(rows, 256, device=gpu_device, dtype=torch.bfloat16)
+
+    def step():
+        y = block(x)
+        return [y.detach()] + list(torch.autograd.grad(y, [x] + params, dy))
+    side = torch.cuda.Stream(gpu_device)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn_like(x))
+            dy.copy_(torch.randn_like(dy))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), i
+
+
+def test_two_graphs_keep_their_own_workspaces(gpu_device):
+    x = [torch.randn(40, 2048, device=gpu_device) for _ in range(2)]
+    w = torch.randn(64, 2048, device=gpu_device) / 45
+    want = [ff.linear(t, w) for t in x]
+    graphs, outs = [], []
+    for t in x:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ff.linear(t, w))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(gpu_device) for _ in x]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+
+
+def test_masked_rows_of_zero_and_large_values(gpu_device):
+    """Rows that are all zero give the bias alone; 16-bit sums that pass the type's largest value become infinite, not wrapped."""
+    w = torch.randn(96, 64, device=gpu_device)
+    b = torch.randn(96, device=gpu_device)
+    y = ff.linear(torch.zeros(33, 64, device=gpu_device), w, b)
+    assert torch.equal(y, b.expand(33, 96))
+    x = torch.full((20, 64), 100.0, device=gpu_device, dtype=torch.float16)
+    y = ff.linear(x, torch.full((40, 64), 100.0, device=gpu_device, dtype=torch.float16))
+    assert torch.isinf(y).all() and (y > 0).all()
+
+
+def test_training_step_of_the_block_follows_the_oracle(gpu_device):
+    """The block under the framework's own optimizer for three steps against the same steps in 64 bits."""
+    from tracknetv3_amd.optim import FusedSGD
+    torch.manual_seed(2)
+    block = ff.GatedFeedForward(64, 176, bias=True).to(gpu_device)
+    ref = {k: v.detach().cpu().double().requires_grad_() for k, v in block.named_parameters()}
+    opt = FusedSGD(block.parameters(), lr=0.05)
+    x, t = torch.randn(48, 64), torch.randn(48, 64)
+    for _ in range(3):
+        opt.zero_grad()
+        ((block(x.to(gpu_device)) - t.to(gpu_device)) ** 2).mean().backward()
+        opt.step()
+        x64 = x.double()
+        g, u = torch.nn.functional.linear(x64, ref["weight"], ref["bias"]).chunk(2, -1)
+        y = torch.nn.functional.linear(torch.nn.functional.silu(g) * u, ref["weight_out"], ref["bias_out"]) + x64
+        grads = torch.autograd.grad(((y - t.double()) ** 2).mean(), list(ref.values()))
+        with torch.no_grad():
+            for p, gr in zip(ref.values(), grads):
+                p -= 0.05 * gr
+    for k, v in block.named_parameters():
+        # three updates of lr * gradient (|gradient| < 1 here), each within fp32's 2^-18 of the gradient's norm, plus the parameter's rounding
+        assert (v.cpu().double() - ref[k]).abs().max() <= 2.0 ** -20, k

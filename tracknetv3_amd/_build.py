@@ -16,7 +16,7 @@ SRC = os.path.join(PKG_DIR, "csrc", "tnv3_capi.hip")
 LIB = os.path.join(PKG_DIR, "libtnv3_hip.so")
 DIAG_LIB = os.path.join(PKG_DIR, "libtnv3_diag.so")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
-FAMILIES = ("MISC", "CONV", "WINO", "WINO43", "UP2X", "WGRAD", "TRAIN")
+FAMILIES = ("MISC", "CONV", "WINO", "WINO43", "UP2X", "WGRAD", "TRAIN", "LINEAR")
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 out of ordinary float code -- some of their forms have given wrong results on this hardware
 # now and then, without an error (the host pass does not know the feature and says so; harmless).
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-cuda-compat",

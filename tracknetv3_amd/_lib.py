@@ -131,6 +131,11 @@ def _declare(lib):
     sig("tnv3_conv1d_k3_dgrad", i, p, p, p, p, i, i, i, i, i, i, p)
     sig("tnv3_conv1d_k3_wgrad_workspace_bytes", sz, i, i, i, i)
     sig("tnv3_conv1d_k3_wgrad", i, p, p, p, p, p, p, sz, i, i, i, i, i, i, p)
+    for kind, extra in (("linear", [p]), ("gated_linear", [])):
+        sig(f"tnv3_{kind}_forward_workspace_bytes", sz, lg, i, i, i)
+        sig(f"tnv3_{kind}_forward", i, p, p, p, *extra, p, p, p, sz, lg, i, i, i, i, p)
+        sig(f"tnv3_{kind}_backward_workspace_bytes", sz, lg, i, i, i, i)
+        sig(f"tnv3_{kind}_backward", i, p, p, p, p, p, p, p, p, sz, lg, i, i, i, i, p)
 
 
 EXPORTS = ["tnv3_abi_version", "tnv3_last_error", "tnv3_conv3x3_num_configs", "tnv3_conv3x3_config_info",
@@ -155,7 +160,10 @@ EXPORTS = ["tnv3_abi_version", "tnv3_last_error", "tnv3_conv3x3_num_configs", "t
            "tnv3_conv3x3_wino_stats_tiles", "tnv3_conv3x3_wino_forward_stats", "tnv3_bn_train_forward_tiles", "tnv3_bn_train_forward_tiles_pool",
            "tnv3_conv3x3_wino_packed_floats", "tnv3_conv3x3_wino_layout", "tnv3_conv3x3_wino_has_stats", "tnv3_conv3x3_wino_pick", "tnv3_conv3x3_wino_supported", "tnv3_conv3x3_wino_pack", "tnv3_conv3x3_wino_pack_view", "tnv3_conv3x3_wino_pack_multi", "tnv3_conv3x3_wino_forward",
            "tnv3_conv3x3_wino43_supported", "tnv3_conv3x3_wino43_packed_floats", "tnv3_conv3x3_wino43_pack", "tnv3_conv3x3_wino43_forward",
-           "tnv3_conv3x3_wino43_stats_tiles", "tnv3_conv3x3_wino43_forward_stats", "tnv3_conv3x3_wino43_dgrad_bnstats"]
+           "tnv3_conv3x3_wino43_stats_tiles", "tnv3_conv3x3_wino43_forward_stats", "tnv3_conv3x3_wino43_dgrad_bnstats",
+           "tnv3_linear_forward_workspace_bytes", "tnv3_linear_forward", "tnv3_linear_backward_workspace_bytes", "tnv3_linear_backward",
+           "tnv3_gated_linear_forward_workspace_bytes", "tnv3_gated_linear_forward", "tnv3_gated_linear_backward_workspace_bytes",
+           "tnv3_gated_linear_backward"]
 
 
 def library_path():

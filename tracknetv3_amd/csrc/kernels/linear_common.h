@@ -1,0 +1,355 @@
+// linear_common.h -- what the position-wise products share (linear, gated_linear and their backward passes): element types, the
+// MFMA 32x32x16 fragments, the activations with their derivatives, and the write-out of a workgroup's tile.
+//
+// Every product is C(i, j) = sum_k A(i, k) B(j, k) with fp32 accumulators:
+//   forward          i = row m of x,      j = output column n,  k = input column:  A = x,   B = W        both k-contiguous
+//   gradient of x    i = row m,           j = input column,     k = output column: A = dz,  B = W^T      B strided in k
+//   gradient of W    i = output column,   j = input column,     k = row m:         A = dz^T, B = x^T     both strided in k
+// MFMA 32x32x16 (16-bit operands): lane l supplies A[l & 31][8 (l >> 5) + 0..7] and B[l & 31][the same k]; accumulator register r of lane l
+// is C[(r & 3) + 8 (r >> 2) + 4 (l >> 5)][l & 31].
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#include "conv3x3_mfma.h"
+
+namespace tnv3 {
+
+typedef short lin_s8 __attribute__((ext_vector_type(8)));
+typedef short lin_s4 __attribute__((ext_vector_type(4)));
+typedef unsigned lin_u4 __attribute__((ext_vector_type(4)));
+
+struct LinBf16 { unsigned short v; };
+struct LinF16 { unsigned short v; };
+
+enum { kLinF32 = 0, kLinBf16 = 1, kLinF16 = 2 };
+enum { kActNone = 0, kActLeaky = 1, kActSigmoid = 2, kActRelu = 3, kActSilu = 4, kActGelu = 5, kActGeluTanh = 6, kActCount = 7 };
+
+#ifndef TNV3_EMU
+typedef __bf16 lin_bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 lin_h8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinBf16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(lin_bf8, a), __builtin_bit_cast(lin_bf8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinF16) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_h8, a), __builtin_bit_cast(lin_h8, b), c, 0, 0, 0);
+}
+// Transposing LDS read: within each group of 16 lanes, lane q's address names 4 elements of row q >> 2 (columns 4 (q & 3) ..), and lane q
+// receives column q of the four rows.
+__device__ __forceinline__ lin_s4 lin_lds_tr4(const unsigned short* p) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) lin_s4*)p);
+}
+// two fp32 -> two 16-bit values, round to nearest even (low half: a)
+__device__ __forceinline__ unsigned lin_pack2(float a, float b, LinBf16) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_convertvector((f2){a, b}, bf2));
+}
+__device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, (h2){(_Float16)a, (_Float16)b});
+}
+__device__ __forceinline__ float lin_f16_up(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
+__device__ __forceinline__ void lin_wave_sync() { __builtin_amdgcn_wave_barrier(); }
+#else
+__device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinBf16) { return emu_mfma_32x32x16(a, b, c, emu_bf16_up); }
+__device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinF16) { return emu_mfma_32x32x16(a, b, c, emu_f16_up); }
+__device__ __forceinline__ lin_s4 lin_lds_tr4(const unsigned short* p) { return emu_lds_tr4(p); }
+__device__ __forceinline__ unsigned lin_pack2(float a, float b, LinBf16) { return (unsigned)emu_bf16_dn(a) | (unsigned)emu_bf16_dn(b) << 16; }
+__device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) { return (unsigned)emu_f16_dn(a) | (unsigned)emu_f16_dn(b) << 16; }
+__device__ __forceinline__ float lin_f16_up(unsigned short h) { return emu_f16_up(h); }
+__device__ __forceinline__ void lin_wave_sync() { emu::wave_barrier(); }
+#endif
+
+__device__ __forceinline__ float lin_bits(unsigned u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ float lin_up(LinBf16 h) { return lin_bits((unsigned)h.v << 16); }
+__device__ __forceinline__ float lin_up(LinF16 h) { return lin_f16_up(h.v); }
+__device__ __forceinline__ float lin_up(float f) { return f; }
+__device__ __forceinline__ void lin_down(float f, LinBf16& o) { o.v = (unsigned short)lin_pack2(f, f, LinBf16{}); }
+__device__ __forceinline__ void lin_down(float f, LinF16& o) { o.v = (unsigned short)lin_pack2(f, f, LinF16{}); }
+__device__ __forceinline__ void lin_down(float f, float& o) { o = f; }
+// the fp32 value that an element of type T keeps of f
+template <class T> __device__ __forceinline__ float lin_round(float f) { T t; lin_down(f, t); return lin_up(t); }
+
+// ---- eight consecutive elements <-> fp32.  vec: p is 16-byte aligned and all eight exist; else the first `n` one by one (the rest 0).
+__device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinBf16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = lin_bits(q[i] << 16); v[2 * i + 1] = lin_bits(q[i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinF16) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = lin_f16_up((unsigned short)(q[i] & 0xffffu)); v[2 * i + 1] = lin_f16_up((unsigned short)(q[i] >> 16)); }
+}
+template <class T> __device__ __forceinline__ void lin_load8(const T* p, float (&v)[8], bool vec, int n) {
+  if (vec) { lin_unpack8(*reinterpret_cast<const lin_u4*>(p), v, T{}); return; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? lin_up(p[i]) : 0.0f;
+}
+template <> __device__ __forceinline__ void lin_load8<float>(const float* p, float (&v)[8], bool vec, int n) {
+  if (vec) {
+    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.0f;
+}
+template <class T> __device__ __forceinline__ void lin_store8(T* p, const float (&v)[8], bool vec, int n) {
+  if (vec) {
+    lin_u4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = lin_pack2(v[2 * i], v[2 * i + 1], T{});
+    *reinterpret_cast<lin_u4*>(p) = q;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) lin_down(v[i], p[i]);
+}
+template <> __device__ __forceinline__ void lin_store8<float>(float* p, const float (&v)[8], bool vec, int n) {
+  if (vec) {
+    reinterpret_cast<f32x4*>(p)[0] = (f32x4){v[0], v[1], v[2], v[3]};
+    reinterpret_cast<f32x4*>(p)[1] = (f32x4){v[4], v[5], v[6], v[7]};
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < n) p[i] = v[i];
+}
+
+// ---- activations.  FAST (16-bit outputs): hardware exp2 and reciprocal, about 2^-21 relative -- an eighth of a percent of the output's own
+// half step; fp32 outputs take the library's expf / erfcf.
+template <bool FAST> __device__ __forceinline__ float lin_exp(float x) { return FAST ? __expf(x) : expf(x); }
+template <bool FAST> __device__ __forceinline__ float lin_rcp(float x) {
+#ifndef TNV3_EMU
+  if (FAST) return __builtin_amdgcn_rcpf(x);
+#endif
+  return 1.0f / x;
+}
+template <bool FAST> __device__ __forceinline__ float lin_sigmoid(float z) { return lin_rcp<FAST>(1.0f + lin_exp<FAST>(-z)); }
+// Phi(z) = erfc(-z / sqrt 2) / 2, the normal distribution.  FAST: the rational form 7.1.26 of Abramowitz & Stegun (1964), |error of erf| <= 1.5e-7.
+template <bool FAST> __device__ __forceinline__ float lin_phi(float z) {
+  if (!FAST) return 0.5f * erfcf(-0.70710678118654752f * z);
+  const float x = 0.70710678118654752f * fabsf(z);
+  const float t = lin_rcp<FAST>(1.0f + 0.3275911f * x);
+  const float p = t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * p * lin_exp<FAST>(-x * x);          // Phi(-|z|)
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+constexpr float kGeluC = 0.79788456080286536f, kGeluA = 0.044715f;
+
+template <bool FAST> __device__ __forceinline__ float lin_act1(float z, int act) {
+  switch (act) {
+    case kActLeaky: return z > 0.0f ? z : 0.01f * z;
+    case kActSigmoid: return lin_sigmoid<FAST>(z);
+    case kActRelu: return z > 0.0f ? z : (z != z ? z : 0.0f);
+    case kActSilu: return z * lin_sigmoid<FAST>(z);
+    case kActGelu: return z * lin_phi<FAST>(z);
+    case kActGeluTanh: return z * lin_sigmoid<FAST>(2.0f * kGeluC * (z + kGeluA * z * z * z));       // (1 + tanh a) / 2 = sigmoid(2 a)
+    default: return z;
+  }
+}
+// (act(z), act'(z)); arguments are clamped to +-64 inside the derivative (NaN kept): beyond it the derivative is 0 or 1 in fp32, and products
+// like z * (1 - sigmoid(z)) would be inf * 0
+template <bool FAST> __device__ __forceinline__ void lin_act_grad1(float z, int act, float& a, float& d) {
+  const float zc = z < -64.0f ? -64.0f : (z > 64.0f ? 64.0f : z);
+  switch (act) {
+    case kActLeaky: a = z > 0.0f ? z : 0.01f * z; d = z > 0.0f ? 1.0f : 0.01f; return;
+    case kActSigmoid: { const float s = lin_sigmoid<FAST>(zc); a = s; d = s * (1.0f - s); return; }
+    case kActRelu: a = z > 0.0f ? z : (z != z ? z : 0.0f); d = z > 0.0f ? 1.0f : 0.0f; return;
+    case kActSilu: { const float s = lin_sigmoid<FAST>(zc); a = z * s; d = s * (1.0f + zc * (1.0f - s)); return; }
+    case kActGelu: { const float p = lin_phi<FAST>(zc); a = z * p; d = p + 0.39894228040143268f * zc * lin_exp<FAST>(-0.5f * zc * zc); return; }
+    case kActGeluTanh: {
+      const float s = lin_sigmoid<FAST>(2.0f * kGeluC * (zc + kGeluA * zc * zc * zc));
+      a = z * s;
+      d = s + 2.0f * zc * s * (1.0f - s) * kGeluC * (1.0f + 3.0f * kGeluA * zc * zc);
+      return;
+    }
+    default: a = z; d = 1.0f; return;
+  }
+}
+template <bool FAST> __device__ __forceinline__ void lin_act8(float (&v)[8], int act) {
+  // the switch is wave-uniform and outside the eight elements' loop
+#define TNV3_LIN_ACT_CASE(A) case A: _Pragma("unroll") for (int i = 0; i < 8; ++i) v[i] = lin_act1<FAST>(v[i], A); break;
+  switch (act) {
+    TNV3_LIN_ACT_CASE(kActLeaky) TNV3_LIN_ACT_CASE(kActSigmoid) TNV3_LIN_ACT_CASE(kActRelu) TNV3_LIN_ACT_CASE(kActSilu)
+    TNV3_LIN_ACT_CASE(kActGelu) TNV3_LIN_ACT_CASE(kActGeluTanh)
+    default: break;
+  }
+#undef TNV3_LIN_ACT_CASE
+}
+
+// ---- one product's arguments
+struct LinGemmArgs {
+  const void* a;          // element (i, k) at a[i * lda + k], or a[k * lda + i] where the kernel's operand is strided in k
+  const void* b;          // element (j, k) likewise
+  long rows_i, rows_j;    // valid i, j (gated: rows_j = the 2 F rows of the weight)
+  long kk;                // contraction length
+  long lda, ldb;
+  const void* bias;       // [rows_j] or null
+  const void* res;        // [rows_i][columns of out] or null
+  void* out;              // [rows_i][rows_j], gated: [rows_i][F]
+  void* pre;              // [rows_i][rows_j]: the pre-activation, for a backward pass; or null
+  float* part;            // splits > 1: [splits][rows_i][rows_j] partial sums instead of all of the above
+  int act;
+  int f;                  // gated: F
+  int tiles_i, tiles_j, splits;
+  long k_per_split;       // a multiple of the kernel's k step
+  int vec;                // bit 0 / 1: a / b can be read in whole 16-byte pieces; bit 2: the outputs (and bias, residual) are such
+};
+enum { kLinVecA = 1, kLinVecB = 2, kLinVecOut = 4 };
+
+// blockIdx -> (tile_i, tile_j, split).  Workgroups go to the 8 XCDs in turn, and each XCD has its own L2: XCD x gets the x-th contiguous
+// eighth of the tile list, and the list walks 8 tiles of i within a panel before the next j, so that the ~32 tiles an XCD works on at a time
+// share 8 panels of A and 4 of B.
+__device__ __forceinline__ void lin_tile(const LinGemmArgs& p, int& ti, int& tj, int& sp) {
+  const int tiles = p.tiles_i * p.tiles_j, total = tiles * p.splits;
+  const int b = blockIdx.x, per = total >> 3, rem = total & 7, x = b & 7;
+  int t = x * per + (x < rem ? x : rem) + (b >> 3);
+  sp = t / tiles;
+  t -= sp * tiles;
+  const int group = 8 * p.tiles_j, g = t / group, in = t - g * group;
+  const int left = p.tiles_i - 8 * g, gh = left < 8 ? left : 8;
+  tj = in / gh;
+  ti = 8 * g + (in - tj * gh);
+}
+
+// ---- write-out of eight consecutive columns of one row; v: fp32 sums (gated: v gate, u the other factor)
+template <class T>
+__device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j, float (&v)[8], const float (&bias)[8]) {
+  if (i >= p.rows_i || j >= p.rows_j) return;
+  const int n = p.rows_j - j < 8 ? (int)(p.rows_j - j) : 8;
+  const bool vec = (p.vec & kLinVecOut) && n == 8;
+  const long o = i * p.rows_j + j;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += bias[e];
+  if (p.pre) lin_store8<T>(static_cast<T*>(p.pre) + o, v, vec, n);
+  lin_act8<sizeof(T) == 2>(v, p.act);
+  if (p.res) {
+    float r[8];
+    lin_load8<T>(static_cast<const T*>(p.res) + o, r, vec, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  }
+  lin_store8<T>(static_cast<T*>(p.out) + o, v, vec, n);
+}
+template <class T>
+__device__ __forceinline__ void lin_finish_gated8(const LinGemmArgs& p, long i, long j, float (&g)[8], float (&u)[8], const float (&bg)[8],
+                                                  const float (&bu)[8]) {
+  if (i >= p.rows_i || j >= p.f) return;
+  const int n = p.f - j < 8 ? (int)(p.f - j) : 8;
+  const bool vec = (p.vec & kLinVecOut) && n == 8;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) { g[e] += bg[e]; u[e] += bu[e]; }
+  if (p.pre) {
+    T* pre = static_cast<T*>(p.pre) + i * p.rows_j + j;
+    lin_store8<T>(pre, g, vec, n);
+    lin_store8<T>(pre + p.f, u, vec, n);
+  }
+  lin_act8<sizeof(T) == 2>(g, p.act);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] *= u[e];
+  lin_store8<T>(static_cast<T*>(p.out) + i * p.f + j, g, vec, n);
+}
+template <class T>
+__device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&b)[8]) {
+  const long left = p.rows_j - j;
+  const int n = left < 8 ? (left < 0 ? 0 : (int)left) : 8;
+  if (p.bias) lin_load8<T>(static_cast<const T*>(p.bias) + (n > 0 ? j : 0), b, (p.vec & kLinVecOut) && n == 8, n);
+  else
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+}
+
+// The write-out goes through LDS, 32 rows x 64 columns per wave at a time (a slab of its own: no workgroup barrier), because the accumulator
+// layout gives a lane one column: read back by rows a lane holds eight consecutive columns, so bias, residual and outputs move in 16-byte pieces.
+// GATED: a wave's first TN/2 column tiles are the gate's, the last TN/2 the other factor's of the same outputs.
+constexpr int kLinSlabLd = 68, kLinSlabFloats = 32 * kLinSlabLd;
+template <class T, int TM, int TN, bool GATED>
+__device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16 (&acc)[TM][TN], float* slab, int lane, long i0, long j0, int sp) {
+  const int half = lane >> 5, col = lane & 31;
+  constexpr int LPR = GATED ? 4 : 8, RPP = 64 / LPR;        // lanes per row, rows per pass
+  const int lr = lane / LPR, c8 = (lane % LPR) * 8;
+#pragma unroll
+  for (int c = 0; c < TN / 2; ++c) {
+    // linear: columns j0 + 64 c ..; gated: outputs j0 + 32 c .. (gate tile c, other factor's tile c + TN / 2)
+    const long j = j0 + (GATED ? 32 * c : 64 * c) + c8;
+    float b0[8], b1[8];
+    if (p.splits == 1) {
+      lin_bias8<T>(p, GATED && j >= p.f ? p.rows_j : j, b0);
+      if (GATED) lin_bias8<T>(p, j >= p.f ? p.rows_j : p.f + j, b1);
+    }
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm) {
+      const f32x16& lo = acc[tm][GATED ? c : 2 * c];
+      const f32x16& hi = acc[tm][GATED ? c + TN / 2 : 2 * c + 1];
+      lin_wave_sync();
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        float* d = slab + ((r & 3) + 8 * (r >> 2) + 4 * half) * kLinSlabLd + col;
+        d[0] = lo[r];
+        d[32] = hi[r];
+      }
+      lin_wave_sync();
+#pragma unroll 1
+      for (int pass = 0; pass < 32 / RPP; ++pass) {
+        const int row = pass * RPP + lr;
+        const float* s = slab + row * kLinSlabLd + c8;
+        float v[8], u[8];
+        lin_load8<float>(s, v, true, 8);
+        if (GATED) lin_load8<float>(s + 32, u, true, 8);
+        const long i = i0 + 32 * tm + row;
+        if (p.splits > 1) {
+          if (i < p.rows_i) {
+            float* part = p.part + ((long)sp * p.rows_i + i) * p.rows_j;
+            const long lim = GATED ? p.f : p.rows_j;
+            const int n = lim - j < 8 ? (int)(lim - j) : 8;
+            const bool vec = (p.vec & kLinVecOut) && n == 8;
+            lin_store8<float>(part + j, v, vec, n);
+            if (GATED) lin_store8<float>(part + p.f + j, u, vec, n);
+          }
+        } else if (GATED) {
+          lin_finish_gated8<T>(p, i, j, v, u, b0, b1);
+        } else {
+          lin_finish8<T>(p, i, j, v, b0);
+        }
+      }
+    }
+  }
+}
+
+// ---- joins the partial sums of a split contraction in a fixed order and finishes them: one work-item per 8 columns of a row
+template <class T, bool GATED>
+__global__ void __launch_bounds__(256) lin_join_kernel(const LinGemmArgs p) {
+  const long cols = GATED ? p.f : p.rows_j, pieces = (cols + 7) / 8;
+  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  const long i = t / pieces, j = (t - i * pieces) * 8;
+  if (i >= p.rows_i) return;
+  const int n = cols - j < 8 ? (int)(cols - j) : 8;
+  const bool vec = (p.vec & kLinVecOut) && n == 8;
+  float v[8], u[8], q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.0f;
+  for (int s = 0; s < p.splits; ++s) {
+    const float* part = p.part + ((long)s * p.rows_i + i) * p.rows_j + j;
+    lin_load8<float>(part, q, vec, n);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += q[e];
+    if (GATED) {
+      lin_load8<float>(part + p.f, q, vec, n);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) u[e] += q[e];
+    }
+  }
+  float b0[8], b1[8];
+  lin_bias8<T>(p, j, b0);
+  if (GATED) {
+    lin_bias8<T>(p, p.f + j, b1);
+    lin_finish_gated8<T>(p, i, j, v, u, b0, b1);
+  } else {
+    lin_finish8<T>(p, i, j, v, b0);
+  }
+}
+
+}  // namespace tnv3

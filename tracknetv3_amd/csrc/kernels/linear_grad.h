@@ -1,0 +1,98 @@
+// linear_grad.h -- the element-wise part of the position-wise layers' backward passes.
+//   linear  dz = dy act'(z)                                       gated  dz = [dh u act'(g) | dh act(g)],  z = [g | u]
+// and the bias gradient, the column sums of dz.  Bound by memory: dy and z are read and dz is written once, in 16-byte pieces.  A workgroup takes 256
+// columns (32 work-items of 8) and every 8th row of its row block per work-item; its column sums are joined through LDS and written as
+// partial sums [row block][columns], which lin_colsum_kernel adds in order: no atomics, the same bits from run to run.
+#pragma once
+#include "linear_common.h"
+
+namespace tnv3 {
+
+struct LinDzArgs {
+  const void* dy;        // [rows][n]
+  const void* pre;       // [rows][n], gated [rows][2 n]; null: no activation, only the column sums are wanted
+  void* dz;              // [rows][n] / [rows][2 n]; null with pre
+  float* part;           // [row blocks][n] / [..][2 n], or null: no bias
+  long rows;
+  int n, act, rows_per_block, vec;
+};
+
+template <class T, bool GATED>
+__global__ void __launch_bounds__(256) lin_dz_kernel(const LinDzArgs p) {
+  constexpr bool FAST = sizeof(T) == 2;
+  __shared__ float red[GATED ? 2 : 1][8][256 + 8];
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const int jt = (p.n + 255) / 256, jb = blockIdx.x % jt;
+  const long rb = blockIdx.x / jt;
+  const int j = jb * 256 + tx * 8, n = p.n - j < 8 ? p.n - j : 8;
+  const bool vec = p.vec && n == 8;
+  const long r0 = rb * p.rows_per_block, r1 = r0 + p.rows_per_block < p.rows ? r0 + p.rows_per_block : p.rows;
+  const int ldz = GATED ? 2 * p.n : p.n;
+  float s0[8], s1[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s0[e] = s1[e] = 0.0f;
+  if (n > 0) {
+    for (long r = r0 + ty; r < r1; r += 8) {
+      float d[8], g[8], u[8];
+      lin_load8<T>(static_cast<const T*>(p.dy) + r * p.n + j, d, vec, n);
+      if (p.pre) {
+        const T* z = static_cast<const T*>(p.pre) + r * ldz + j;
+        T* o = static_cast<T*>(p.dz) + r * ldz + j;
+        lin_load8<T>(z, g, vec, n);
+        if (GATED) lin_load8<T>(z + p.n, u, vec, n);
+        // the switch outside of the eight elements' loop; the column sums take dz before it is rounded to T
+#define TNV3_LIN_DZ_CASE(A)                                              \
+  case A:                                                                \
+    _Pragma("unroll") for (int e = 0; e < 8; ++e) {                      \
+      float av, dv;                                                      \
+      lin_act_grad1<FAST>(g[e], A, av, dv);                              \
+      if (GATED) { g[e] = d[e] * u[e] * dv; u[e] = d[e] * av; }          \
+      else g[e] = d[e] * dv;                                             \
+    }                                                                    \
+    break;
+        switch (p.act) {
+          TNV3_LIN_DZ_CASE(kActLeaky) TNV3_LIN_DZ_CASE(kActSigmoid) TNV3_LIN_DZ_CASE(kActRelu) TNV3_LIN_DZ_CASE(kActSilu)
+          TNV3_LIN_DZ_CASE(kActGelu) TNV3_LIN_DZ_CASE(kActGeluTanh)
+          default:
+            TNV3_LIN_DZ_CASE(kActNone)
+        }
+#undef TNV3_LIN_DZ_CASE
+        lin_store8<T>(o, g, vec, n);
+        if (GATED) lin_store8<T>(o + p.n, u, vec, n);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { s0[e] += g[e]; if (GATED) s1[e] += u[e]; }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s0[e] += d[e];
+      }
+    }
+  }
+  if (!p.part) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    red[0][ty][tx * 8 + e] = s0[e];
+    if (GATED) red[GATED ? 1 : 0][ty][tx * 8 + e] = s1[e];
+  }
+  __syncthreads();
+  const int c = threadIdx.x, col = jb * 256 + c;
+  if (col >= p.n) return;
+#pragma unroll
+  for (int h = 0; h < (GATED ? 2 : 1); ++h) {
+    float s = 0.0f;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) s += red[h][y][c];
+    p.part[rb * ldz + h * p.n + col] = s;
+  }
+}
+
+// out[j] = sum over the row blocks, in order
+template <class T>
+__global__ void __launch_bounds__(256) lin_colsum_kernel(const float* __restrict__ part, T* __restrict__ out, int n, int blocks) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= n) return;
+  float s = 0.0f;
+  for (int b = 0; b < blocks; ++b) s += part[(long)b * n + j];
+  lin_down(s, out[j]);
+}
+
+}  // namespace tnv3

@@ -1,0 +1,128 @@
+"""Position-wise layers with gradients: `linear` (matrix product with bias, activation and residual in its epilogue), `gated_linear` (both
+projections of a gated feed-forward block, activation and product in one kernel) and the modules built from them.
+
+They stand beside InpaintNet's Conv1d + activation layers (reference model.py:76-87) and the 1x1 head (model.py:45), for rows of any width in
+fp32, bf16 or fp16.  `x` is (..., k) with any leading shape, one position per row: InpaintNet's (N, L, C) sequences go in as they are.
+
+    from tracknetv3_amd.feedforward import GatedFeedForward
+    block = GatedFeedForward(256, 704).to("cuda", torch.bfloat16)
+    y = block(x)                                  # x + W_out (silu(W_gate x) * W_up x)
+
+Gradients are exact to the type: the pre-activation is kept in the tensors' type for the backward pass, sums are fp32.
+"""
+import math
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+ACTIVATIONS = {"none": ops.ACT_NONE, "leaky_relu": ops.ACT_LEAKY_RELU, "sigmoid": ops.ACT_SIGMOID, "relu": ops.ACT_RELU, "silu": ops.ACT_SILU,
+               "gelu": ops.ACT_GELU, "gelu_tanh": ops.ACT_GELU_TANH}
+
+
+def _act(act):
+    if isinstance(act, str):
+        if act not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+        return ACTIVATIONS[act]
+    return act
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act):
+        y, pre = ops.linear(x, weight, bias, residual, act, want_pre=True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, pre = ctx.saved_tensors
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            dx, dw, db = ops.linear_backward(dy.contiguous(), x, weight, pre, ctx.act, (need_x, need_w, need_b))
+        return dx, dw, db, (dy if need_r else None), None
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act):
+        h, pre = ops.gated_linear(x, weight, bias, act, want_pre=True)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act = act
+        return h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x, weight, pre = ctx.saved_tensors
+        dx, dw, db = ops.gated_linear_backward(dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad[:3])
+        return dx, dw, db, None
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def linear(x, weight, bias=None, residual=None, act="none"):
+    """act(x weight^T + bias) + residual; x (..., k), weight (n, k), bias (n,), residual (..., n), all of one type.  act: a name of ACTIVATIONS
+    or an ops.ACT_* constant.  Differentiable in every tensor."""
+    act = _act(act)
+    x, weight, bias, residual = _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual)
+    if _wants_grad(x, weight, bias, residual):
+        return _Linear.apply(x, weight, bias, residual, act)
+    return ops.linear(x, weight, bias, residual, act)
+
+
+def gated_linear(x, weight, bias=None, act="silu"):
+    """act(g) * u with [g | u] = x weight^T + bias; x (..., k), weight (2 n, k) with the gate's n rows first, bias (2 n,).  Differentiable in every
+    tensor."""
+    act = _act(act)
+    x, weight, bias = _contiguous(x), _contiguous(weight), _contiguous(bias)
+    if _wants_grad(x, weight, bias):
+        return _GatedLinear.apply(x, weight, bias, act)
+    return ops.gated_linear(x, weight, bias, act)
+
+
+class Linear(nn.Linear):
+    """nn.Linear (same parameters and state_dict) with an activation and a residual in the product's epilogue."""
+
+    def __init__(self, in_features, out_features, bias=True, act="none", device=None, dtype=None):
+        super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
+        _act(act)
+        self.act = act
+
+    def forward(self, x, residual=None):
+        return linear(x, self.weight, self.bias, residual, self.act)
+
+
+class GatedFeedForward(nn.Module):
+    """y = W_out (act(W_gate x + b_gate) * (W_up x + b_up)) + b_out [+ x].  weight (2 hidden, dim) holds W_gate's rows, then W_up's."""
+
+    def __init__(self, dim, hidden, act="silu", bias=False, residual=True, device=None, dtype=None):
+        super().__init__()
+        _act(act)
+        kw = {"device": device, "dtype": dtype}
+        self.dim, self.hidden, self.act, self.residual = int(dim), int(hidden), act, bool(residual)
+        self.weight = nn.Parameter(torch.empty(2 * self.hidden, self.dim, **kw))
+        self.weight_out = nn.Parameter(torch.empty(self.dim, self.hidden, **kw))
+        self.bias = nn.Parameter(torch.empty(2 * self.hidden, **kw)) if bias else None
+        self.bias_out = nn.Parameter(torch.empty(self.dim, **kw)) if bias else None
+        for p, fan_in in ((self.weight, self.dim), (self.bias, self.dim), (self.weight_out, self.hidden), (self.bias_out, self.hidden)):
+            if p is not None:
+                nn.init.uniform_(p, -1 / math.sqrt(fan_in), 1 / math.sqrt(fan_in))      # nn.Linear's range
+
+    def forward(self, x):
+        if x.shape[-1] != self.dim:
+            raise ValueError(f"GatedFeedForward expects (..., {self.dim}), got {tuple(x.shape)}")
+        h = gated_linear(x, self.weight, self.bias, self.act)
+        return linear(h, self.weight_out, self.bias_out, x if self.residual else None)

@@ -1158,6 +1158,109 @@ def conv1d_k3_wgrad(src0, dpre, src1=None, src_nlc=False):
     return dw, db
 
 
+# ------------------------------------------------------------------------------------------------- position-wise layers
+ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 3, 4, 5, 6
+_LINEAR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _linear_args(what, x, weight, bias, others, gated):
+    """(rows, k, n, dtype code) of a position-wise layer's call after its checks; others: (name, tensor or None, shape) of the same type."""
+    code = _LINEAR_DTYPES.get(x.dtype)
+    if code is None:
+        raise _lib.Tnv3Error(f"{what}: expected float32, bfloat16 or float16, got {x.dtype}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise _lib.Tnv3Error(f"{what}: weight {tuple(weight.shape)} does not match inputs of shape {tuple(x.shape)}")
+    n2, k = weight.shape
+    if k == 0 or n2 == 0 or (gated and n2 % 2):
+        raise _lib.Tnv3Error(f"{what}: bad weight shape {tuple(weight.shape)}" + (" (gated: an even number of rows)" if gated else ""))
+    if bias is not None and tuple(bias.shape) != (n2,):
+        raise _lib.Tnv3Error(f"{what}: bias of shape {tuple(bias.shape)}, expected ({n2},)")
+    for name, t, shape in others:
+        if t is not None and tuple(t.shape) != tuple(shape):
+            raise _lib.Tnv3Error(f"{what}: {name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
+    tensors = (x, weight, bias) + tuple(t for _, t, _ in others)
+    for t in tensors:
+        if t is not None and t.dtype != x.dtype:
+            raise _lib.Tnv3Error(f"{what}: all tensors must be {x.dtype}, got {t.dtype}")
+    _lib.dev_check(*tensors)
+    return x.numel() // k, k, n2 // 2 if gated else n2, code
+
+
+def _linear_act(what, act):
+    act = int(act)
+    if not ACT_NONE <= act <= ACT_GELU_TANH:
+        raise _lib.Tnv3Error(f"{what}: unknown activation {act}")
+    return act
+
+
+def linear(x, weight, bias=None, residual=None, act=ACT_NONE, want_pre=False):
+    """act(x weight^T + bias) + residual for x (..., k), weight (n, k) (tnv3_linear_forward); fp32, bf16 or fp16, fp32 sums.  want_pre: returns
+    (y, pre) -- pre, the pre-activation that linear_backward takes (None for ACT_NONE)."""
+    lib = _lib.load()
+    act = _linear_act("linear", act)
+    rows, k, n, code = _linear_args("linear", x, weight, bias, (("residual", residual, x.shape[:-1] + weight.shape[:1]),), False)
+    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    pre = torch.empty_like(y) if want_pre and act != ACT_NONE else None
+    if rows:
+        need = lib.tnv3_linear_forward_workspace_bytes(rows, k, n, code)
+        ws = _workspace(need, x.device) if need else None
+        _lib.check(lib.tnv3_linear_forward(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(residual), _lib.ptr(y), _lib.ptr(pre), _lib.ptr(ws),
+                                           need, rows, k, n, act, code, _lib.stream_ptr(x)))
+    return (y, pre) if want_pre else y
+
+
+def gated_linear(x, weight, bias=None, act=ACT_SILU, want_pre=False):
+    """act(g) * u with [g | u] = x weight^T + bias for x (..., k), weight (2 n, k) -- the gate's n rows first (tnv3_gated_linear_forward).
+    want_pre: returns (h, pre (..., 2 n)), what gated_linear_backward takes."""
+    lib = _lib.load()
+    act = _linear_act("gated_linear", act)
+    rows, k, n, code = _linear_args("gated_linear", x, weight, bias, (), True)
+    h = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=x.dtype, device=x.device) if want_pre else None
+    if rows:
+        need = lib.tnv3_gated_linear_forward_workspace_bytes(rows, k, n, code)
+        ws = _workspace(need, x.device) if need else None
+        _lib.check(lib.tnv3_gated_linear_forward(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(h), _lib.ptr(pre), _lib.ptr(ws), need, rows,
+                                                 k, n, act, code, _lib.stream_ptr(x)))
+    return (h, pre) if want_pre else h
+
+
+def _linear_backward(what, gated, dy, x, weight, pre, act, want):
+    lib = _lib.load()
+    act = _linear_act(what, act)
+    wide = x.shape[:-1] + weight.shape[:1]
+    out = x.shape[:-1] + (weight.shape[0] // 2,) if gated else wide
+    needs_pre = gated or act != ACT_NONE
+    if needs_pre and pre is None:
+        raise _lib.Tnv3Error(f"{what}: the forward's pre-activation is required")
+    rows, k, n, code = _linear_args(what, x, weight, None, (("upstream gradient", dy, out), ("pre", pre if needs_pre else None, wide)), gated)
+    n2 = int(weight.shape[0])
+    if rows == 0:
+        return (torch.empty_like(x) if want[0] else None, torch.zeros_like(weight) if want[1] else None,
+                torch.zeros(n2, dtype=x.dtype, device=x.device) if want[2] else None)
+    dx = torch.empty_like(x) if want[0] else None
+    dw = torch.empty_like(weight) if want[1] else None
+    db = torch.empty(n2, dtype=x.dtype, device=x.device) if want[2] else None
+    query = lib.tnv3_gated_linear_backward_workspace_bytes if gated else lib.tnv3_linear_backward_workspace_bytes
+    call = lib.tnv3_gated_linear_backward if gated else lib.tnv3_linear_backward
+    need = query(rows, k, n, act, code)
+    ws = _workspace(need, x.device)
+    _lib.check(call(_lib.ptr(dy), _lib.ptr(x), _lib.ptr(weight), _lib.ptr(pre if needs_pre else None), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws),
+                    need, rows, k, n, act, code, _lib.stream_ptr(x)))
+    return dx, dw, db
+
+
+def linear_backward(dy, x, weight, pre=None, act=ACT_NONE, want=(True, True, True)):
+    """(dx, dweight, dbias) of linear for the upstream gradient dy (the residual's gradient is dy itself); want: which of the three to compute
+    (the others are None).  pre: linear(..., want_pre=True)'s second result."""
+    return _linear_backward("linear_backward", False, dy, x, weight, pre, act, want)
+
+
+def gated_linear_backward(dh, x, weight, pre, act=ACT_SILU, want=(True, True, True)):
+    """(dx, dweight, dbias) of gated_linear for the upstream gradient dh; pre: gated_linear(..., want_pre=True)'s second result."""
+    return _linear_backward("gated_linear_backward", True, dh, x, weight, pre, act, want)
+
+
 # ------------------------------------------------------------------------------------------------- device guard
 # The C ABI runs a call on its stream's device, but a tensor's *default* stream is the NULL stream (= "the calling thread's
 # current device"), and the stream-less workspace queries plan for the current device too.  Every op therefore runs with the
@@ -1167,7 +1270,8 @@ _TENSOR_OPS = ["pack_conv3x3_weights", "bn_eval_scale", "pack_wino_weights", "pa
                "heatmap_peakfind", "heatmap_box_max", "bn_train_forward", "bn_relu_backward", "bn_bwd_consts", "conv3x3_wino_dgrad_bnstats", "bn_relu_backward_tiles", "conv3x3_dgrad", "conv3x3_wgrad",
                "conv3x3_wgrad_wino", "conv3x3_wgrad_up2x", "wbce_forward", "wbce_backward", "head_backward", "head1x1_sigmoid_wbce", "head_wbce_backward",
                "maxpool2x2_backward_add", "maxpool2x2_backward_add_bnstats", "dgrad_up2x_wino_bnstats", "maxpool2x2_bnstats_supported", "upsample2x_backward", "mixup", "conv1d_act_backward", "conv1d_k3_dgrad", "conv1d_k3_wgrad",
-               "grad_norm", "adam_step", "sgd_step", "inpaintnet_pack", "inpaintnet_pack_t", "inpaintnet_fused_train_forward", "inpaintnet_fused_backward"]          # list-of-tensor ops: the guard looks inside the lists
+               "grad_norm", "adam_step", "sgd_step", "inpaintnet_pack", "inpaintnet_pack_t", "inpaintnet_fused_train_forward", "inpaintnet_fused_backward",
+               "linear", "gated_linear", "linear_backward", "gated_linear_backward"]          # list-of-tensor ops: the guard looks inside the lists
 for _name in _TENSOR_OPS:
     globals()[_name] = _lib.on_tensor_device(globals()[_name])
 del _name
