@@ -40,6 +40,18 @@ def test_split_contraction_joins_all_parts(emu, monkeypatch):
         lc.check_exact(40, 1100, 24, dtype, True, True, False, "cpu")
 
 
+@pytest.mark.parametrize("lazy", ["0", "1"])
+@pytest.mark.parametrize("cus", ["1", "256"])
+def test_direct_loads_land_before_they_are_read(emu, monkeypatch, cus, lazy):
+    """16-bit operands that move by direct loads: pieces landing as early or as late as the program's waits allow; one CU makes the wide tiles
+    the choice."""
+    monkeypatch.setenv("TNV3_EMU_CUS", cus)
+    monkeypatch.setenv("TNV3_EMU_LAZY_DMA", lazy)
+    for dtype in (torch.bfloat16, torch.float16):
+        lc.check_exact(70, 200, 264, dtype, False, True, True, "cpu")
+        lc.check_exact(130, 264, 136, dtype, True, True, False, "cpu")
+
+
 def test_fp32_keeps_infinities_and_nan_where_they_belong(emu):
     inf, nan = float("inf"), float("nan")
     x = torch.randn(5, 40)

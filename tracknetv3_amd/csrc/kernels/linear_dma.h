@@ -1,0 +1,156 @@
+// linear_dma.h -- the wide products of 16-bit operands: tiles move from memory to LDS by direct loads, nothing passes through registers on the way.
+//
+// A workgroup of WM x WN waves computes (TM 32 WM) x (TN 32 WN) outputs, 64 of the contraction per step, two LDS stages.  A wave owns TM x TN MFMA tiles.
+// One barrier per step, placed before the LAST quarter of a step's products: at that point every wave has the step's last fragments in
+// registers and its share of the next stage has landed, so behind the barrier the stage just read can be refilled (a whole step for the loads to
+// arrive) and the next step's first fragments are read under the last quarter's products.  No product waits for a read that was not issued a
+// quarter step (8 or 4 MFMAs of 32 cycles per wave, two waves per SIMD) earlier.
+#pragma once
+#include "linear_common.h"
+#include "linear_staged.h"
+
+namespace tnv3 {
+
+template <int TM_, int TN_, int WM_, int WN_>
+struct LinDmaCfg {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
+  static constexpr int NW = WM * WN, NT = NW * 64, BI = TM * 32 * WM, BJ = TN * 32 * WN, BK = 64;
+  static constexpr int STAGE = (BI + BJ) * BK;                                  // 16-bit elements
+  static constexpr int SLABS = NW * kLinSlabFloats * 2;
+  static constexpr int LDS = 2 * STAGE > SLABS ? 2 * STAGE : SLABS;
+};
+
+// One operand's direct loads: a wave moves ROWS / 8 / NW pieces of 1 KB per step (64 lanes x 16 bytes, consecutive in LDS; the lane picks the chunk
+// that belongs there).  k-contiguous: 8 rows of 64; k-strided: 512 / ROWS rows of k.
+template <bool KS, int ROWS, int NW>
+struct LinDma {
+  static constexpr int N = ROWS / 8 / NW;
+  static_assert(N * 8 * NW == ROWS, "whole pieces per wave");
+  unsigned off[N];          // bytes from the operand's first element of the step
+  int kchunk;               // k-contiguous: first k of the lane's chunk
+  const char* base;
+  long left;                // bytes from base to the operand's end
+  long step;                // bytes per step
+  // base_el: the tile's first element; end_el: the operand's element count; row_off: rows to add to this wave's pieces
+  __device__ __forceinline__ void init(const void* src, long base_el, long end_el, long ld, int wave, int lane) {
+    base = static_cast<const char*>(src) + 2 * base_el;
+    left = 2 * (end_el - base_el);
+    step = KS ? 128 * ld : 128;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int piece = wave * N + i;
+      if (KS) {
+        constexpr int LPR = ROWS / 8;
+        const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((k & 3) << 1);
+        off[i] = (unsigned)(k * (int)(2 * ld) + c * 16);
+      } else {
+        const int r = lane >> 3, c = (lane & 7) ^ r;
+        off[i] = (unsigned)((piece * 8 + r) * (int)(2 * ld) + c * 16);
+        kchunk = c * 8;
+      }
+    }
+  }
+  // kleft: elements of the contraction left in this split from the step's first on
+  __device__ __forceinline__ void issue(unsigned short* tile, long kleft, int wave) {
+    const unsigned bytes = left <= 0 ? 0u : (left > 0x7fffffffl ? 0x7fffffffu : (unsigned)left);
+    const tnv3_rsrc_t r = tnv3_make_rsrc(base, bytes);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      tnv3_buf_dma16(r, reinterpret_cast<float*>(tile + (wave * N + i) * 512), !KS && kchunk >= kleft ? kDmaOob : off[i]);
+    base += step;
+    left -= step;
+  }
+};
+
+__device__ __forceinline__ void lin_dma_sync() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0): this wave's loads have landed, its fragments are in registers
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <class Cfg, class T, bool KSA, bool KSB, bool GATED>
+__global__ void __launch_bounds__(Cfg::NT, 2) lin_dma_kernel(const LinGemmArgs p) {
+  constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, STAGE = Cfg::STAGE, Q = BK / 16;
+  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / Cfg::WN, wj = wave % Cfg::WN;
+  int ti, tj, sp;
+  lin_tile(p, ti, tj, sp);
+  const long i0 = (long)ti * BI, j0 = (long)tj * (GATED ? BJ / 2 : BJ);
+  const long kbeg = (long)sp * p.k_per_split, kend = kbeg + p.k_per_split < p.kk ? kbeg + p.k_per_split : p.kk;
+  const int steps = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
+
+  LinDma<KSA, BI, Cfg::NW> da;
+  LinDma<KSB, BJ, Cfg::NW> db;
+  da.init(p.a, KSA ? kbeg * p.lda + i0 : i0 * p.lda + kbeg, KSA ? p.kk * p.lda : p.rows_i * p.lda, p.lda, wave, lane);
+  if (GATED) {
+    // tile row r holds weight row (r / H odd ? f : 0) + j0 + (r / 2H) H + r % H, H = TN 16: a wave's pieces lie in one run of H rows, so the jump is
+    // in its base
+    constexpr int H = TN * 16, N8 = LinDma<KSB, BJ, Cfg::NW>::N * 8;
+    static_assert(!GATED || H % N8 == 0, "a wave's pieces stay within one half");
+    const int r0 = wave * N8, run = r0 / H;
+    const long row = j0 + (long)(run >> 1) * H + (run & 1 ? p.f : 0) - (long)run * H;        // so that base + r0 rows is the wave's first row
+    db.init(p.b, row * p.ldb + kbeg, p.rows_j * p.ldb, p.ldb, wave, lane);
+  } else {
+    db.init(p.b, KSB ? kbeg * p.ldb + j0 : j0 * p.ldb + kbeg, KSB ? p.kk * p.ldb : p.rows_j * p.ldb, p.ldb, wave, lane);
+  }
+  long kleft = kend - kbeg;
+  auto dma = [&](int s) {
+    unsigned short* t = lds + (s & 1) * STAGE;
+    da.issue(t, kleft, wave);
+    db.issue(t + BI * BK, kleft, wave);
+    kleft -= BK;
+  };
+
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int x = 0; x < TM; ++x)
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+
+  lin_s8 fa[2][TM], fb[2][TN];
+  auto read = [&](int s, int q, int set) {
+    const unsigned short* t = lds + (s & 1) * STAGE;
+#pragma unroll
+    for (int x = 0; x < TM; ++x) fa[set][x] = lin_frag<KSA, BK, BI>(t, wi * TM * 32, x, q, lane);
+#pragma unroll
+    for (int y = 0; y < TN; ++y) fb[set][y] = lin_frag<KSB, BK, BJ>(t + BI * BK, wj * TN * 32, y, q, lane);
+  };
+  auto products = [&](int set) {
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+#pragma unroll
+      for (int x = 0; x < TM; ++x) acc[x][y] = lin_mfma(fa[set][x], fb[set][y], acc[x][y], T{});
+  };
+
+  if (steps > 0) {
+    dma(0);
+    lin_dma_sync();
+    if (steps > 1) dma(1);
+    read(0, 0, 0);
+  }
+  for (int s = 0; s < steps; ++s) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+      if (q + 1 < Q) {
+        read(s, q + 1, (q + 1) & 1);
+      } else {
+        lin_dma_sync();
+        if (s + 2 < steps) dma(s + 2);
+        if (s + 1 < steps) read(s + 1, 0, 0);
+      }
+      // (the fences keep the reads ahead of the products: left alone, the scheduler puts each read right in front of its use)
+      __builtin_amdgcn_sched_barrier(0);
+      products(q & 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  lin_dma_sync();
+  lin_write_out<T, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
+                                  j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
+}
+
+}  // namespace tnv3

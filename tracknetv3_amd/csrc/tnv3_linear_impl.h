@@ -1,6 +1,7 @@
 // tnv3_linear_impl.h -- argument checks, workspaces and dispatch of the position-wise layers (tnv3_linear_*, tnv3_gated_linear_*).
 #pragma once
 #include "kernels/linear_common.h"
+#include "kernels/linear_dma.h"
 #include "kernels/linear_grad.h"
 #include "kernels/linear_staged.h"
 #include "tnv3_impl.h"
@@ -8,6 +9,8 @@
 namespace tnv3 {
 
 using LinS128 = LinStagedCfg<2, 2, 2, 2>;       // 128 x 128, four waves of 64 x 64
+using LinD256 = LinDmaCfg<2, 4, 4, 2>;          // 256 x 256, eight waves of 64 x 128: one workgroup per CU
+using LinD128 = LinDmaCfg<2, 2, 2, 2>;          // 128 x 128, four waves of 64 x 64: two workgroups per CU
 
 constexpr long kLinMaxWidth = 1l << 20;         // columns: a tile's rows stay within 2^31 bytes of its first
 constexpr long kLinMaxRows = 1l << 30;
@@ -26,6 +29,11 @@ struct LinPlan {
 inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated) {
   LinPlan pl;
   pl.bi = pl.bj = 128;
+  // 16-bit products with at least a 256 x 256 tile for every CU take those: half the LDS and L2 traffic per product
+  if (dtype != kLinF32) {
+    const long big = ((rows_i + 255) / 256) * (gated ? (rows_j / 2 + 127) / 128 : (rows_j + 255) / 256);
+    if (big >= num_cus()) pl.bi = pl.bj = 256;
+  }
   const long ti = (rows_i + pl.bi - 1) / pl.bi, tj = gated ? (rows_j / 2 + pl.bj / 2 - 1) / (pl.bj / 2) : (rows_j + pl.bj - 1) / pl.bj;
   const long tiles = ti * tj, cus = num_cus(), step = 64, steps = (kk + step - 1) / step;
   // fewer tiles than CUs: the contraction is split so that all take part, as long as a part keeps 4 steps of 64
@@ -48,11 +56,20 @@ template <class T, bool KSA, bool KSB, bool GATED, class Launcher>
 int lin_launch(Launcher& L, LinGemmArgs& p, const LinPlan& pl) {
   p.splits = pl.splits;
   p.k_per_split = pl.k_per_split;
-  p.tiles_i = (int)((p.rows_i + pl.bi - 1) / pl.bi);
-  p.tiles_j = GATED ? (p.f + pl.bj / 2 - 1) / (pl.bj / 2) : (int)((p.rows_j + pl.bj - 1) / pl.bj);
+  const bool direct = sizeof(T) == 2 && (p.vec & kLinVecA) && (p.vec & kLinVecB);
+  const int bi = direct ? pl.bi : 128, bj = direct ? pl.bj : 128;
+  p.tiles_i = (int)((p.rows_i + bi - 1) / bi);
+  p.tiles_j = GATED ? (p.f + bj / 2 - 1) / (bj / 2) : (int)((p.rows_j + bj - 1) / bj);
   const long grid = (long)p.tiles_i * p.tiles_j * p.splits;
   if (grid >= (1l << 31)) TNV3_FAIL(-1, "linear: %ld tiles are more than one launch takes", grid);
-  int rc = L.launch(lin_staged_kernel<LinS128, T, KSA, KSB, GATED>, (int)grid, LinS128::NT, p);
+  int rc;
+  if constexpr (sizeof(T) == 2) {
+    if (direct && bi == 256) rc = L.launch(lin_dma_kernel<LinD256, T, KSA, KSB, GATED>, (int)grid, LinD256::NT, p);
+    else if (direct) rc = L.launch(lin_dma_kernel<LinD128, T, KSA, KSB, GATED>, (int)grid, LinD128::NT, p);
+    else rc = L.launch(lin_staged_kernel<LinS128, T, KSA, KSB, GATED>, (int)grid, LinS128::NT, p);
+  } else {
+    rc = L.launch(lin_staged_kernel<LinS128, T, KSA, KSB, GATED>, (int)grid, LinS128::NT, p);
+  }
   if (rc || p.splits == 1) return rc;
   const long pieces = p.rows_i * (((GATED ? p.f : p.rows_j) + 7) / 8), blocks = (pieces + 255) / 256;
   if (blocks >= (1l << 31)) TNV3_FAIL(-1, "linear: %ld workgroups are more than one launch takes", blocks);
