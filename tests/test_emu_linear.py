@@ -47,12 +47,14 @@ def test_direct_loads_land_before_they_are_read(emu, monkeypatch, cus, lazy):
     the choice."""
     monkeypatch.setenv("TNV3_EMU_CUS", cus)
     monkeypatch.setenv("TNV3_EMU_LAZY_DMA", lazy)
-    for dtype in (torch.bfloat16, torch.float16):
+    for dtype in lc.DTYPES:
         lc.check_exact(70, 200, 264, dtype, False, True, True, "cpu")
         lc.check_exact(130, 264, 136, dtype, True, True, False, "cpu")
 
 
-def test_fp32_keeps_infinities_and_nan_where_they_belong(emu):
+@pytest.mark.parametrize("cus", ["1", "256"])
+def test_fp32_keeps_infinities_and_nan_where_they_belong(emu, monkeypatch, cus):
+    monkeypatch.setenv("TNV3_EMU_CUS", cus)
     inf, nan = float("inf"), float("nan")
     x = torch.randn(5, 40)
     w = torch.randn(6, 40)

@@ -51,6 +51,10 @@ __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) {
 }
 __device__ __forceinline__ float lin_f16_up(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
 __device__ __forceinline__ void lin_wave_sync() { __builtin_amdgcn_wave_barrier(); }
+// four fp32 at base + voffset + soffset, each checked against the descriptor's range (beyond it: 0)
+__device__ __forceinline__ f32x4 lin_buf_load4(tnv3_rsrc_t r, unsigned voffset, unsigned soffset) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(voffset + soffset), 0, 0));
+}
 #else
 __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinBf16) { return emu_mfma_32x32x16(a, b, c, emu_bf16_up); }
 __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinF16) { return emu_mfma_32x32x16(a, b, c, emu_f16_up); }
@@ -59,6 +63,16 @@ __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinBf16) { retur
 __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) { return (unsigned)emu_f16_dn(a) | (unsigned)emu_f16_dn(b) << 16; }
 __device__ __forceinline__ float lin_f16_up(unsigned short h) { return emu_f16_up(h); }
 __device__ __forceinline__ void lin_wave_sync() { emu::wave_barrier(); }
+__device__ __forceinline__ f32x4 lin_buf_load4(tnv3_rsrc_t r, unsigned voffset, unsigned soffset) {
+  f32x4 v;
+  for (int e = 0; e < 4; ++e) {
+    const unsigned long long o = (unsigned long long)voffset + soffset + 4 * e;
+    float f = 0.0f;
+    if (o + 4 <= r.num_records) memcpy(&f, r.base + o, 4);
+    v[e] = f;
+  }
+  return v;
+}
 #endif
 
 __device__ __forceinline__ float lin_bits(unsigned u) { return __builtin_bit_cast(float, u); }
@@ -268,6 +282,7 @@ __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&
 constexpr int kLinSlabLd = 68, kLinSlabFloats = 32 * kLinSlabLd;
 template <class T, int TM, int TN, bool GATED>
 __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16 (&acc)[TM][TN], float* slab, int lane, long i0, long j0, int sp) {
+  static_assert(TN % 2 == 0, "a slab is two column tiles wide");
   const int half = lane >> 5, col = lane & 31;
   constexpr int LPR = GATED ? 4 : 8, RPP = 64 / LPR;        // lanes per row, rows per pass
   const int lr = lane / LPR, c8 = (lane % LPR) * 8;

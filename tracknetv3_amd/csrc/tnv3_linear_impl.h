@@ -3,6 +3,7 @@
 #include "kernels/linear_common.h"
 #include "kernels/linear_dma.h"
 #include "kernels/linear_grad.h"
+#include "kernels/linear_split.h"
 #include "kernels/linear_staged.h"
 #include "tnv3_impl.h"
 
@@ -11,6 +12,8 @@ namespace tnv3 {
 using LinS128 = LinStagedCfg<2, 2, 2, 2>;       // 128 x 128, four waves of 64 x 64
 using LinD256 = LinDmaCfg<2, 4, 4, 2>;          // 256 x 256, eight waves of 64 x 128: one workgroup per CU
 using LinD128 = LinDmaCfg<2, 2, 2, 2>;          // 128 x 128, four waves of 64 x 64: two workgroups per CU
+using LinF256 = LinSplitCfg<2, 2, 4, 2>;        // fp32: 256 x 128, eight waves of 64 x 64, one workgroup per CU (144 KB of LDS)
+using LinF128 = LinSplitCfg<1, 2, 4, 1>;        // fp32: 128 x 64, four waves of 32 x 64, two workgroups per CU
 
 constexpr long kLinMaxWidth = 1l << 20;         // columns: a tile's rows stay within 2^31 bytes of its first
 constexpr long kLinMaxRows = 1l << 30;
@@ -29,6 +32,11 @@ struct LinPlan {
 inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated) {
   LinPlan pl;
   pl.bi = pl.bj = 128;
+  if (dtype == kLinF32) {
+    const long big = ((rows_i + 255) / 256) * (gated ? (rows_j / 2 + 63) / 64 : (rows_j + 127) / 128);
+    if (big >= num_cus()) pl.bi = 256;
+    else pl.bj = 64;
+  }
   // 16-bit products with at least a 256 x 256 tile for every CU take those: half the LDS and L2 traffic per product
   if (dtype != kLinF32) {
     const long big = ((rows_i + 255) / 256) * (gated ? (rows_j / 2 + 127) / 128 : (rows_j + 255) / 256);
@@ -57,7 +65,7 @@ int lin_launch(Launcher& L, LinGemmArgs& p, const LinPlan& pl) {
   p.splits = pl.splits;
   p.k_per_split = pl.k_per_split;
   const bool direct = sizeof(T) == 2 && (p.vec & kLinVecA) && (p.vec & kLinVecB);
-  const int bi = direct ? pl.bi : 128, bj = direct ? pl.bj : 128;
+  const int bi = direct || sizeof(T) == 4 ? pl.bi : 128, bj = direct || sizeof(T) == 4 ? pl.bj : 128;
   p.tiles_i = (int)((p.rows_i + bi - 1) / bi);
   p.tiles_j = GATED ? (p.f + bj / 2 - 1) / (bj / 2) : (int)((p.rows_j + bj - 1) / bj);
   const long grid = (long)p.tiles_i * p.tiles_j * p.splits;
@@ -68,7 +76,8 @@ int lin_launch(Launcher& L, LinGemmArgs& p, const LinPlan& pl) {
     else if (direct) rc = L.launch(lin_dma_kernel<LinD128, T, KSA, KSB, GATED>, (int)grid, LinD128::NT, p);
     else rc = L.launch(lin_staged_kernel<LinS128, T, KSA, KSB, GATED>, (int)grid, LinS128::NT, p);
   } else {
-    rc = L.launch(lin_staged_kernel<LinS128, T, KSA, KSB, GATED>, (int)grid, LinS128::NT, p);
+    if (bi == 256) rc = L.launch(lin_split_kernel<LinF256, KSA, KSB, GATED>, (int)grid, LinF256::NT, p);
+    else rc = L.launch(lin_split_kernel<LinF128, KSA, KSB, GATED>, (int)grid, LinF128::NT, p);
   }
   if (rc || p.splits == 1) return rc;
   const long pieces = p.rows_i * (((GATED ? p.f : p.rows_j) + 7) / 8), blocks = (pieces + 255) / 256;
