@@ -66,7 +66,7 @@ def bounds(x, w, b, r, act, gated, dy, dtype):
     if dy is None:
         return out
     d = dy.cpu().double().abs().reshape(y.shape)
-    ezs = ez + u * z + tiny                                  # of the pre-activation as it is kept
+    ezs = ez + (2.0 ** -24 if gated else u) * z + tiny       # of the pre-activation as it is kept: fp32 / the type
     if gated:
         g, uu = z.chunk(2, -1)
         eg, eu = ezs.chunk(2, -1)

@@ -204,7 +204,7 @@ struct LinGemmArgs {
   const void* bias;       // [rows_j] or null
   const void* res;        // [rows_i][columns of out] or null
   void* out;              // [rows_i][rows_j], gated: [rows_i][F]
-  void* pre;              // [rows_i][rows_j]: the pre-activation, for a backward pass; or null
+  void* pre;              // [rows_i][rows_j]: the pre-activation, for a backward pass, or null; gated: fp32 whatever the type
   float* part;            // splits > 1: [splits][rows_i][rows_j] partial sums instead of all of the above
   int act;
   int f;                  // gated: F
@@ -257,9 +257,9 @@ __device__ __forceinline__ void lin_finish_gated8(const LinGemmArgs& p, long i, 
 #pragma unroll
   for (int e = 0; e < 8; ++e) { g[e] += bg[e]; u[e] += bu[e]; }
   if (p.pre) {
-    T* pre = static_cast<T*>(p.pre) + i * p.rows_j + j;
-    lin_store8<T>(pre, g, vec, n);
-    lin_store8<T>(pre + p.f, u, vec, n);
+    float* pre = static_cast<float*>(p.pre) + i * p.rows_j + j;
+    lin_store8<float>(pre, g, vec, n);
+    lin_store8<float>(pre + p.f, u, vec, n);
   }
   lin_act8<sizeof(T) == 2>(g, p.act);
 #pragma unroll

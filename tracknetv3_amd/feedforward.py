@@ -8,7 +8,7 @@ fp32, bf16 or fp16.  `x` is (..., k) with any leading shape, one position per ro
     block = GatedFeedForward(256, 704).to("cuda", torch.bfloat16)
     y = block(x)                                  # x + W_out (silu(W_gate x) * W_up x)
 
-Gradients are exact to the type: the pre-activation is kept in the tensors' type for the backward pass, sums are fp32.
+The pre-activation is kept for the backward pass -- linear's in the tensors' type, gated_linear's in fp32 -- and sums are fp32.
 """
 import math
 

@@ -1211,12 +1211,12 @@ def linear(x, weight, bias=None, residual=None, act=ACT_NONE, want_pre=False):
 
 def gated_linear(x, weight, bias=None, act=ACT_SILU, want_pre=False):
     """act(g) * u with [g | u] = x weight^T + bias for x (..., k), weight (2 n, k) -- the gate's n rows first (tnv3_gated_linear_forward).
-    want_pre: returns (h, pre (..., 2 n)), what gated_linear_backward takes."""
+    want_pre: returns (h, pre) -- the fp32 pre-activations (..., 2 n) that gated_linear_backward takes."""
     lib = _lib.load()
     act = _linear_act("gated_linear", act)
     rows, k, n, code = _linear_args("gated_linear", x, weight, bias, (), True)
     h = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=x.dtype, device=x.device) if want_pre else None
+    pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=torch.float32, device=x.device) if want_pre else None
     if rows:
         need = lib.tnv3_gated_linear_forward_workspace_bytes(rows, k, n, code)
         ws = _workspace(need, x.device) if need else None
@@ -1233,7 +1233,12 @@ def _linear_backward(what, gated, dy, x, weight, pre, act, want):
     needs_pre = gated or act != ACT_NONE
     if needs_pre and pre is None:
         raise _lib.Tnv3Error(f"{what}: the forward's pre-activation is required")
-    rows, k, n, code = _linear_args(what, x, weight, None, (("upstream gradient", dy, out), ("pre", pre if needs_pre else None, wide)), gated)
+    rows, k, n, code = _linear_args(what, x, weight, None, (("upstream gradient", dy, out), ("pre", pre if needs_pre and not gated else None, wide)), gated)
+    if gated:
+        _f32(pre)
+        _lib.dev_check(x, pre)
+        if pre.shape != wide:
+            raise _lib.Tnv3Error(f"{what}: pre of shape {tuple(pre.shape)}, expected {tuple(wide)}")
     n2 = int(weight.shape[0])
     if rows == 0:
         return (torch.empty_like(x) if want[0] else None, torch.zeros_like(weight) if want[1] else None,
