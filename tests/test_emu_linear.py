@@ -11,7 +11,7 @@ from tracknetv3_amd import _lib, feedforward as ff, ops
 
 @pytest.mark.parametrize("dtype", lc.DTYPES)
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 64, 32), (3, 5, 7), (17, 72, 40), (33, 129, 65), (130, 40, 136)])
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 64, 32), (3, 5, 7), (17, 72, 40), (33, 129, 65), (5, 200, 20), (66, 70, 33), (130, 40, 136)])
 def test_exact_integers(emu, rows, k, n, gated, dtype):
     lc.check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device="cpu", seed=rows + k)
 
@@ -34,10 +34,10 @@ def test_no_bias_no_residual_and_leading_shape(emu):
 def test_split_contraction_joins_all_parts(emu, monkeypatch):
     """Few rows and a long contraction: the parts' partial sums are joined."""
     lib = _lib.load()
-    assert lib.tnv3_linear_forward_workspace_bytes(40, 1100, 24, 0) > 0
+    assert lib.tnv3_linear_forward_workspace_bytes(70, 1100, 24, 0) > 0
     for dtype in lc.DTYPES:
-        lc.check_exact(40, 1100, 24, dtype, False, True, True, "cpu")
-        lc.check_exact(40, 1100, 24, dtype, True, True, False, "cpu")
+        lc.check_exact(70, 1100, 24, dtype, False, True, True, "cpu")
+        lc.check_exact(70, 1100, 24, dtype, True, True, False, "cpu")
 
 
 @pytest.mark.parametrize("lazy", ["0", "1"])
@@ -164,10 +164,10 @@ def test_refusals(emu):
                 dict(dtype=3), dict(xp=null)):
         assert fwd(**bad) != 0, bad
     assert lib.tnv3_linear_backward(p(y), p(x), p(w), null, p(x), null, null, null, 0, 4, 8, 6, 0, 0, null) != 0           # no workspace
-    long_k = lib.tnv3_linear_forward_workspace_bytes(40, 1100, 24, 0)
-    big = [torch.zeros(s) for s in ((40, 1100), (24, 1100), (40, 24))]
+    long_k = lib.tnv3_linear_forward_workspace_bytes(70, 1100, 24, 0)
+    big = [torch.zeros(s) for s in ((70, 1100), (24, 1100), (70, 24))]
     ws = torch.zeros(long_k // 4)
     args = [p(big[0]), p(big[1]), null, null, p(big[2]), null]
-    assert lib.tnv3_linear_forward(*args, p(ws), long_k - 4, 40, 1100, 24, 0, 0, null) != 0                                  # too small
-    assert lib.tnv3_linear_forward(*args, p(ws), long_k, 40, 1100, 24, 0, 0, null) == 0
+    assert lib.tnv3_linear_forward(*args, p(ws), long_k - 4, 70, 1100, 24, 0, 0, null) != 0                                  # too small
+    assert lib.tnv3_linear_forward(*args, p(ws), long_k, 70, 1100, 24, 0, 0, null) == 0
     assert lib.tnv3_linear_forward_workspace_bytes(0, 1, 1, 0) == 0

@@ -19,6 +19,9 @@ typedef short lin_s8 __attribute__((ext_vector_type(8)));
 typedef short lin_s4 __attribute__((ext_vector_type(4)));
 typedef unsigned lin_u4 __attribute__((ext_vector_type(4)));
 
+template <bool V> struct LinFlag { static constexpr bool value = V; };
+template <int V> struct LinCount { static constexpr int value = V; };
+
 struct LinBf16 { unsigned short v; };
 struct LinF16 { unsigned short v; };
 

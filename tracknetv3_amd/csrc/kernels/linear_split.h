@@ -103,8 +103,6 @@ struct LinSplitLoader {
   }
 };
 
-template <bool V> struct LinFlag { static constexpr bool value = V; };
-
 template <class Cfg, bool KSA, bool KSB, bool GATED>
 __global__ void __launch_bounds__(Cfg::NT, 2) lin_split_kernel(const LinGemmArgs p) {
   constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, NT = Cfg::NT, STAGE = Cfg::STAGE;

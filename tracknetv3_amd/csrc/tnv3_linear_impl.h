@@ -3,6 +3,7 @@
 #include "kernels/linear_common.h"
 #include "kernels/linear_dma.h"
 #include "kernels/linear_grad.h"
+#include "kernels/linear_rows.h"
 #include "kernels/linear_split.h"
 #include "kernels/linear_staged.h"
 #include "tnv3_impl.h"
@@ -85,6 +86,17 @@ int lin_launch(Launcher& L, LinGemmArgs& p, const LinPlan& pl) {
   return L.launch(lin_join_kernel<T, GATED>, (int)blocks, 256, p);
 }
 
+// Forward products of up to kLinFewRows rows.
+constexpr long kLinFewRows = 64;
+template <class T, bool GATED, class Launcher>
+int lin_rows_launch(Launcher& L, LinGemmArgs& p) {
+  p.splits = 1;
+  const int grid = (int)(((GATED ? (long)p.f : p.rows_j) + 15) / 16);
+  if (p.rows_i <= 16) return L.launch(lin_rows_kernel<T, 1, 16, GATED>, grid, 1024, p);
+  if (p.rows_i <= 32) return L.launch(lin_rows_kernel<T, 2, 8, GATED>, grid, 512, p);
+  return L.launch(lin_rows_kernel<T, 4, 8, GATED>, grid, 512, p);
+}
+
 // ---- the three products of a layer (n2: rows of the weight)
 template <class T, bool GATED, class Launcher>
 int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const void* bias, const void* res, void* out, void* pre, void* ws, long rows,
@@ -97,6 +109,7 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   const bool kvec = k % e16 == 0;
   p.vec = (kvec && lin_aligned(x) ? kLinVecA : 0) | (kvec && lin_aligned(w) ? kLinVecB : 0) |
           (n % 8 == 0 && lin_aligned(bias) && lin_aligned(res) && lin_aligned(out) && lin_aligned(pre) ? kLinVecOut : 0);
+  if (rows <= kLinFewRows) return lin_rows_launch<T, GATED>(L, p);
   return lin_launch<T, false, false, GATED>(L, p, lin_plan(dtype, rows, n2, k, GATED));
 }
 template <class T, class Launcher>
@@ -146,7 +159,7 @@ inline int lin_check(const char* what, long rows, int k, int n, int act, int dty
 
 inline size_t lin_forward_workspace_bytes(long rows, int k, int n, int dtype, bool gated) {
   if (lin_check("workspace", rows, k, n, 0, dtype, gated)) return 0;
-  return lin_plan(dtype, rows, gated ? 2l * n : n, k, gated).part_bytes;
+  return rows <= kLinFewRows ? 0 : lin_plan(dtype, rows, gated ? 2l * n : n, k, gated).part_bytes;
 }
 struct LinBackwardLayout { size_t dz, sums, part, total; };
 inline LinBackwardLayout lin_backward_layout(long rows, int k, int n, int act, int dtype, bool gated) {

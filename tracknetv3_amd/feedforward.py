@@ -30,6 +30,8 @@ def _act(act):
     return act
 
 
+# (The backward passes call the ops' unchecked form: every tensor is the forward's own or has the shape and type that autograd guarantees, on the
+# device that autograd made current.)
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
@@ -42,11 +44,13 @@ class _Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, pre = ctx.saved_tensors
-        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        need = ctx.needs_input_grad
         dx = dw = db = None
-        if need_x or need_w or need_b:
-            dx, dw, db = ops.linear_backward(dy.contiguous(), x, weight, pre, ctx.act, (need_x, need_w, need_b))
-        return dx, dw, db, (dy if need_r else None), None
+        if need[0] or need[1] or need[2]:
+            n, k = weight.shape
+            dx, dw, db = ops._linear_backward_call(False, dy if dy.is_contiguous() else dy.contiguous(), x, weight, pre, ctx.act, need, x.numel() // k, k, n,
+                                                   ops._LINEAR_DTYPES[x.dtype])
+        return dx, dw, db, (dy if need[3] else None), None
 
 
 class _GatedLinear(torch.autograd.Function):
@@ -61,24 +65,21 @@ class _GatedLinear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh):
         x, weight, pre = ctx.saved_tensors
-        dx, dw, db = ops.gated_linear_backward(dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad[:3])
-        return dx, dw, db, None
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-def _contiguous(t):
-    return t if t is None or t.is_contiguous() else t.contiguous()
+        n2, k = weight.shape
+        return ops._linear_backward_call(True, dh if dh.is_contiguous() else dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad, x.numel() // k, k,
+                                         n2 // 2, ops._LINEAR_DTYPES[x.dtype]) + (None,)
 
 
 def linear(x, weight, bias=None, residual=None, act="none"):
     """act(x weight^T + bias) + residual; x (..., k), weight (n, k), bias (n,), residual (..., n), all of one type.  act: a name of ACTIVATIONS
     or an ops.ACT_* constant.  Differentiable in every tensor."""
     act = _act(act)
-    x, weight, bias, residual = _contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual)
-    if _wants_grad(x, weight, bias, residual):
+    x = x if x.is_contiguous() else x.contiguous()
+    weight = weight if weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    residual = residual if residual is None or residual.is_contiguous() else residual.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
+                                    (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
     return ops.linear(x, weight, bias, residual, act)
 
@@ -87,8 +88,10 @@ def gated_linear(x, weight, bias=None, act="silu"):
     """act(g) * u with [g | u] = x weight^T + bias; x (..., k), weight (2 n, k) with the gate's n rows first, bias (2 n,).  Differentiable in every
     tensor."""
     act = _act(act)
-    x, weight, bias = _contiguous(x), _contiguous(weight), _contiguous(bias)
-    if _wants_grad(x, weight, bias):
+    x = x if x.is_contiguous() else x.contiguous()
+    weight = weight if weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, act)
     return ops.gated_linear(x, weight, bias, act)
 

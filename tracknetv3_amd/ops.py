@@ -1159,53 +1159,81 @@ def conv1d_k3_wgrad(src0, dpre, src1=None, src_nlc=False):
 
 
 # ------------------------------------------------------------------------------------------------- position-wise layers
+# Small calls are bound by what the host does: the checks below look at each tensor once, and the workspace sizes are looked up.
 ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 3, 4, 5, 6
 _LINEAR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_LINEAR_WORKSPACE = {}          # (entry, device, sizes ..) -> bytes: a pure function of its key
 
 
-def _linear_args(what, x, weight, bias, others, gated):
-    """(rows, k, n, dtype code) of a position-wise layer's call after its checks; others: (name, tensor or None, shape) of the same type."""
+def _linear_check(what, x, weight, bias, act, gated):
+    """(rows, k, n, dtype code) of a position-wise layer's call after its checks."""
     code = _LINEAR_DTYPES.get(x.dtype)
     if code is None:
         raise _lib.Tnv3Error(f"{what}: expected float32, bfloat16 or float16, got {x.dtype}")
+    if not isinstance(act, int) or not ACT_NONE <= act <= ACT_GELU_TANH:
+        raise _lib.Tnv3Error(f"{what}: unknown activation {act!r}")
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
         raise _lib.Tnv3Error(f"{what}: weight {tuple(weight.shape)} does not match inputs of shape {tuple(x.shape)}")
     n2, k = weight.shape
     if k == 0 or n2 == 0 or (gated and n2 % 2):
         raise _lib.Tnv3Error(f"{what}: bad weight shape {tuple(weight.shape)}" + (" (gated: an even number of rows)" if gated else ""))
-    if bias is not None and tuple(bias.shape) != (n2,):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n2):
         raise _lib.Tnv3Error(f"{what}: bias of shape {tuple(bias.shape)}, expected ({n2},)")
-    for name, t, shape in others:
-        if t is not None and tuple(t.shape) != tuple(shape):
-            raise _lib.Tnv3Error(f"{what}: {name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
-    tensors = (x, weight, bias) + tuple(t for _, t, _ in others)
-    for t in tensors:
-        if t is not None and t.dtype != x.dtype:
-            raise _lib.Tnv3Error(f"{what}: all tensors must be {x.dtype}, got {t.dtype}")
-    _lib.dev_check(*tensors)
+    _linear_tensor(what, "weight", weight, x, x.dtype)
+    if bias is not None:
+        _linear_tensor(what, "bias", bias, x, x.dtype)
+    if not x.is_contiguous():
+        raise _lib.Tnv3Error("tnv3 ops need contiguous tensors")
+    if not x.is_cuda and not _lib.is_emulator():
+        raise _lib.Tnv3Error("tnv3 ops run on the GPU only (tensor is on %s); there is no CPU fallback" % x.device)
     return x.numel() // k, k, n2 // 2 if gated else n2, code
 
 
-def _linear_act(what, act):
-    act = int(act)
-    if not ACT_NONE <= act <= ACT_GELU_TANH:
-        raise _lib.Tnv3Error(f"{what}: unknown activation {act}")
-    return act
+def _linear_tensor(what, name, t, x, dtype, shape=None):
+    if shape is not None and t.shape != shape:
+        raise _lib.Tnv3Error(f"{what}: {name} of shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise _lib.Tnv3Error(f"{what}: {name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise _lib.Tnv3Error("tnv3 ops need contiguous tensors")
+    if t.get_device() != x.get_device():
+        raise _lib.Tnv3Error(f"tensors on different devices: {x.device} vs {t.device}")
+
+
+def _linear_workspace(lib, entry, x, *sizes):
+    """(scratch tensor or None, bytes) for one call."""
+    if _lib.is_emulator():
+        need = getattr(lib, entry)(*sizes)
+    else:
+        key = (entry, x.get_device()) + sizes
+        need = _LINEAR_WORKSPACE.get(key)
+        if need is None:
+            need = _LINEAR_WORKSPACE[key] = getattr(lib, entry)(*sizes)
+    return (torch.empty((need + 7) // 8, dtype=torch.int64, device=x.device), need) if need else (None, 0)
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _linear_stream(x):
+    return torch._C._cuda_getCurrentRawStream(x.get_device()) if x.is_cuda else 0
 
 
 def linear(x, weight, bias=None, residual=None, act=ACT_NONE, want_pre=False):
     """act(x weight^T + bias) + residual for x (..., k), weight (n, k) (tnv3_linear_forward); fp32, bf16 or fp16, fp32 sums.  want_pre: returns
     (y, pre) -- pre, the pre-activation that linear_backward takes (None for ACT_NONE)."""
     lib = _lib.load()
-    act = _linear_act("linear", act)
-    rows, k, n, code = _linear_args("linear", x, weight, bias, (("residual", residual, x.shape[:-1] + weight.shape[:1]),), False)
-    y = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
+    rows, k, n, code = _linear_check("linear", x, weight, bias, act, False)
+    shape = x.shape[:-1] + (n,)
+    if residual is not None:
+        _linear_tensor("linear", "residual", residual, x, x.dtype, shape)
+    y = torch.empty(shape, dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre and act != ACT_NONE else None
     if rows:
-        need = lib.tnv3_linear_forward_workspace_bytes(rows, k, n, code)
-        ws = _workspace(need, x.device) if need else None
-        _lib.check(lib.tnv3_linear_forward(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(residual), _lib.ptr(y), _lib.ptr(pre), _lib.ptr(ws),
-                                           need, rows, k, n, act, code, _lib.stream_ptr(x)))
+        ws, need = _linear_workspace(lib, "tnv3_linear_forward_workspace_bytes", x, rows, k, n, code)
+        _lib.check(lib.tnv3_linear_forward(x.data_ptr(), weight.data_ptr(), _address(bias), _address(residual), y.data_ptr(), _address(pre), _address(ws),
+                                           need, rows, k, n, act, code, _linear_stream(x)))
     return (y, pre) if want_pre else y
 
 
@@ -1213,45 +1241,42 @@ def gated_linear(x, weight, bias=None, act=ACT_SILU, want_pre=False):
     """act(g) * u with [g | u] = x weight^T + bias for x (..., k), weight (2 n, k) -- the gate's n rows first (tnv3_gated_linear_forward).
     want_pre: returns (h, pre) -- the fp32 pre-activations (..., 2 n) that gated_linear_backward takes."""
     lib = _lib.load()
-    act = _linear_act("gated_linear", act)
-    rows, k, n, code = _linear_args("gated_linear", x, weight, bias, (), True)
+    rows, k, n, code = _linear_check("gated_linear", x, weight, bias, act, True)
     h = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
     pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=torch.float32, device=x.device) if want_pre else None
     if rows:
-        need = lib.tnv3_gated_linear_forward_workspace_bytes(rows, k, n, code)
-        ws = _workspace(need, x.device) if need else None
-        _lib.check(lib.tnv3_gated_linear_forward(_lib.ptr(x), _lib.ptr(weight), _lib.ptr(bias), _lib.ptr(h), _lib.ptr(pre), _lib.ptr(ws), need, rows,
-                                                 k, n, act, code, _lib.stream_ptr(x)))
+        ws, need = _linear_workspace(lib, "tnv3_gated_linear_forward_workspace_bytes", x, rows, k, n, code)
+        _lib.check(lib.tnv3_gated_linear_forward(x.data_ptr(), weight.data_ptr(), _address(bias), h.data_ptr(), _address(pre), _address(ws), need, rows,
+                                                 k, n, act, code, _linear_stream(x)))
     return (h, pre) if want_pre else h
 
 
 def _linear_backward(what, gated, dy, x, weight, pre, act, want):
+    rows, k, n, code = _linear_check(what, x, weight, None, act, gated)
+    _linear_tensor(what, "upstream gradient", dy, x, x.dtype, x.shape[:-1] + (n,))
+    if gated or act != ACT_NONE:
+        if pre is None:
+            raise _lib.Tnv3Error(f"{what}: the forward's pre-activation is required")
+        _linear_tensor(what, "pre", pre, x, torch.float32 if gated else x.dtype, x.shape[:-1] + weight.shape[:1])
+    else:
+        pre = None
+    return _linear_backward_call(gated, dy, x, weight, pre, act, want, rows, k, n, code)
+
+
+def _linear_backward_call(gated, dy, x, weight, pre, act, want, rows, k, n, code):
     lib = _lib.load()
-    act = _linear_act(what, act)
-    wide = x.shape[:-1] + weight.shape[:1]
-    out = x.shape[:-1] + (weight.shape[0] // 2,) if gated else wide
-    needs_pre = gated or act != ACT_NONE
-    if needs_pre and pre is None:
-        raise _lib.Tnv3Error(f"{what}: the forward's pre-activation is required")
-    rows, k, n, code = _linear_args(what, x, weight, None, (("upstream gradient", dy, out), ("pre", pre if needs_pre and not gated else None, wide)), gated)
-    if gated:
-        _f32(pre)
-        _lib.dev_check(x, pre)
-        if pre.shape != wide:
-            raise _lib.Tnv3Error(f"{what}: pre of shape {tuple(pre.shape)}, expected {tuple(wide)}")
-    n2 = int(weight.shape[0])
+    n2 = 2 * n if gated else n
     if rows == 0:
         return (torch.empty_like(x) if want[0] else None, torch.zeros_like(weight) if want[1] else None,
                 torch.zeros(n2, dtype=x.dtype, device=x.device) if want[2] else None)
     dx = torch.empty_like(x) if want[0] else None
     dw = torch.empty_like(weight) if want[1] else None
     db = torch.empty(n2, dtype=x.dtype, device=x.device) if want[2] else None
-    query = lib.tnv3_gated_linear_backward_workspace_bytes if gated else lib.tnv3_linear_backward_workspace_bytes
+    ws, need = _linear_workspace(lib, "tnv3_gated_linear_backward_workspace_bytes" if gated else "tnv3_linear_backward_workspace_bytes", x, rows, k, n,
+                                 act, code)
     call = lib.tnv3_gated_linear_backward if gated else lib.tnv3_linear_backward
-    need = query(rows, k, n, act, code)
-    ws = _workspace(need, x.device)
-    _lib.check(call(_lib.ptr(dy), _lib.ptr(x), _lib.ptr(weight), _lib.ptr(pre if needs_pre else None), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), _lib.ptr(ws),
-                    need, rows, k, n, act, code, _lib.stream_ptr(x)))
+    _lib.check(call(dy.data_ptr(), x.data_ptr(), weight.data_ptr(), _address(pre), _address(dx), _address(dw), _address(db), _address(ws), need, rows, k, n,
+                    act, code, _linear_stream(x)))
     return dx, dw, db
 
 
