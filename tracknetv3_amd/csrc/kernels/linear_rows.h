@@ -1,12 +1,12 @@
 // linear_rows.h -- forward products of few rows (single positions of a stream, small batches): bound by reading the weight once.
 //
 // A workgroup takes 16 weight rows (gated: 16 of the gate and the same 16 of the other factor) against all rows of x; its NW waves share the
-// contraction, 128 bytes of every row per wave in turn, and join their sums through LDS in a fixed order.  Operands go from memory straight into MFMA
-// fragments (16x16x32 for 16-bit types, 16x16x4 for fp32): each weight element is used once, so there is nothing for LDS to share, and x is small
-// enough to stay in L2.  Each lane's 16-byte loads need no alignment beyond the element's: odd widths run at the same speed.  fp32 stays on the fp32
-// matrix pipe -- its 157 TFLOP/s are far above what the weight's bytes allow here.
-// Four blocks of loads are issued before the first is used (96 of the 128 registers that 16 waves per CU leave each), so that a CU has
-// 64 KB and more in flight.
+// contraction, one block of 128 bytes per row each in turn, and join their sums through LDS in a fixed order.  A block goes through registers and a
+// piece of LDS of the wave's own (no barrier): 8 lanes load a row's 128 bytes, which the fragment reads (16x16x32 MFMA for 16-bit types, 16x16x4 for
+// fp32) then take apart.  Loaded straight into fragments, 16 neighbouring lanes would name 16 different cache lines and the CU's address path would
+// be the bound (16 bytes per clock: 1 x 4096 -> 8192 in bf16 14.0 us, 64 rows 37.9 us).  The 16-byte loads need no alignment beyond the element's: odd
+// widths take the same path.  fp32 stays on the fp32 matrix pipe, whose rate is far above what the weight's bytes allow here.
+// U blocks of loads are issued before the first is used, and a block's registers are loaded again as soon as they are free.
 #pragma once
 #include "linear_common.h"
 
@@ -63,75 +63,108 @@ template <class T> __device__ __forceinline__ lin_u4 lin_load_first(const T* row
 
 template <class T, int MT, int NW, bool GATED>
 __global__ void __launch_bounds__(NW * 64) lin_rows_kernel(const LinGemmArgs p) {
-  constexpr int EL = 16 / (int)sizeof(T), BLK = 8 * EL, G = GATED ? 2 : 1, U = MT * G >= 4 ? 1 : (MT * G == 2 ? 2 : 4);
-  __shared__ __attribute__((aligned(16))) float red[NW][G][MT][256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, kq = (lane >> 4) * EL;
+  constexpr int EL = 16 / (int)sizeof(T), BLK = 8 * EL, G = GATED ? 2 : 1, U = MT * G == 1 ? 4 : (MT * G < 8 ? 2 : 1);
+  constexpr int WROWS = 16 * G, ROWS = WROWS + 16 * MT, NWL = WROWS / 8, NL = ROWS / 8;        // staged rows; loads (8 rows each) per block
+  constexpr int STAGE = NW * ROWS * 32, RED = NW * G * MT * 256;                               // floats
+  __shared__ __attribute__((aligned(1024))) float lds[STAGE > RED ? STAGE : RED];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15;
+  const int lr = lane >> 3, piece = lane & 7;
   const long n0 = (long)blockIdx.x * 16, nout = GATED ? p.f : p.rows_j;
+  float* stage = lds + wave * ROWS * 32;
 
-  const T* wp[G];
-  const T* xp[MT];
-  // rows beyond the last repeat it: their results are not written
-  const long wr = n0 + r16 < nout ? n0 + r16 : nout - 1;
+  // the lane's 16 bytes of each load: row 8 i + lane / 8 (weight rows, then x rows; beyond the last: the last again, results not written), piece
+  // lane & 7.  Groups of 8 x rows that do not exist are not loaded at all.
+  unsigned off[NL];                                   // bytes from the uniform base of the row group (below 64 rows x 2^20 x 4)
 #pragma unroll
-  for (int g = 0; g < G; ++g) wp[g] = static_cast<const T*>(p.b) + (wr + (g ? p.f : 0)) * p.ldb + kq;
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const long xr = 16 * m + r16 < p.rows_i ? 16 * m + r16 : p.rows_i - 1;
-    xp[m] = static_cast<const T*>(p.a) + xr * p.lda + kq;
+  for (int i = 0; i < NL; ++i) {
+    const int r = (i < NWL ? i & 1 : i - NWL) * 8 + lr;
+    const long last = (i < NWL ? nout - n0 : p.rows_i) - 1;
+    off[i] = (unsigned)(r < last ? r : last) * (unsigned)(sizeof(T) * (i < NWL ? p.ldb : p.lda)) + piece * 16;
   }
+  const char* base[3] = {reinterpret_cast<const char*>(static_cast<const T*>(p.b) + n0 * p.ldb),
+                         reinterpret_cast<const char*>(static_cast<const T*>(p.b) + (n0 + p.f) * p.ldb), static_cast<const char*>(p.a)};
+  auto src = [&](int i) -> const char* { return base[i < NWL ? i >> 1 : 2]; };
+  const int xgroups = (int)((p.rows_i + 7) / 8);
   f32x4 acc[G][MT];
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[g][m] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-  const int nfull = (int)(p.kk / BLK), tail = (int)(p.kk % BLK);
-  auto run = [&](int b, auto count) {
-    constexpr int C = decltype(count)::value;
-    lin_u4 w[C][2][G], x[C][2][MT];
+  lin_u4 v[U][NL];
+  auto load = [&](int c, int t) {
 #pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long k = (long)(b + c * NW) * BLK + h * 4 * EL;
-#pragma unroll
-        for (int g = 0; g < G; ++g) w[c][h][g] = *reinterpret_cast<const lin_u4_any*>(wp[g] + k);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) x[c][h][m] = *reinterpret_cast<const lin_u4_any*>(xp[m] + k);
-      }
-    __builtin_amdgcn_sched_barrier(0);           // all loads of the blocks are issued before the first product
-#pragma unroll
-    for (int c = 0; c < C; ++c)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int g = 0; g < G; ++g)
-#pragma unroll
-          for (int m = 0; m < MT; ++m) acc[g][m] = lin_mfma16(w[c][h][g], x[c][h][m], acc[g][m], T{});
+    for (int i = 0; i < NL; ++i)
+      if (i < NWL || i - NWL < xgroups) v[c][i] = *reinterpret_cast<const lin_u4_any*>(src(i) + (long)t * 128 + off[i]);
   };
-  int b = wave;
-  for (; b + (U - 1) * NW < nfull; b += U * NW) run(b, LinCount<U>{});
-  for (; b < nfull; b += NW) run(b, LinCount<1>{});
-  if (tail && nfull % NW == wave) {
-    // what whole blocks leave over: the row's last block, without the elements that were summed already; rows shorter than a block: one by one
-    const int skip = (int)p.kk - BLK;
+  auto put = [&](int c) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      auto part = [&](const T* lane_row) -> lin_u4 {
-        if (nfull) return lin_keep_from<T>(*reinterpret_cast<const lin_u4_any*>(lane_row + skip + h * 4 * EL), BLK - tail - h * 4 * EL - kq);
-        return lin_load_first<T>(lane_row - kq, lane_row + h * 4 * EL, tail - h * 4 * EL - kq);
-      };
-      lin_u4 x[MT];
+    for (int i = 0; i < NL; ++i)
+      if (i < NWL || i - NWL < xgroups) *reinterpret_cast<lin_u4*>(stage + (8 * i + lr) * 32 + ((piece ^ lr) << 2)) = v[c][i];
+  };
+  auto use = [&]() {
+    lin_wave_sync();
+    lin_u4 f[2][ROWS / 16];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) x[m] = part(xp[m]);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int g = 0; g < G; ++g) {
-        const lin_u4 w = part(wp[g]);
+      for (int q = 0; q < ROWS / 16; ++q)
+        f[h][q] = *reinterpret_cast<const lin_u4*>(stage + (16 * q + r16) * 32 + ((((lane >> 4) + 4 * h) ^ (r16 & 7)) << 2));
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[g][m] = lin_mfma16(w, x[m], acc[g][m], T{});
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[g][m] = lin_mfma16(f[h][g], f[h][G + m], acc[g][m], T{});
+    lin_wave_sync();
+  };
+  const int nfull = (int)(p.kk / BLK), tail = (int)(p.kk % BLK);
+  const int mine = nfull > wave ? (nfull - wave + NW - 1) / NW : 0;        // this wave's whole blocks: wave, wave + NW, ..
+  int t = wave, left = mine;
+  if (left >= U) {
+#pragma unroll
+    for (int c = 0; c < U; ++c) load(c, t + c * NW);
+    t += U * NW;
+    left -= U;
+    for (; left >= U; left -= U, t += U * NW) {
+#pragma unroll
+      for (int c = 0; c < U; ++c) {
+        put(c);
+        load(c, t + c * NW);
+        use();
       }
     }
+#pragma unroll
+    for (int c = 0; c < U; ++c) {
+      put(c);
+      use();
+    }
   }
+  if (left > 0) {                                     // fewer than U blocks: all their loads first
+#pragma unroll
+    for (int c = 0; c < U - 1; ++c)
+      if (c < left) load(c, t + c * NW);
+#pragma unroll
+    for (int c = 0; c < U - 1; ++c)
+      if (c < left) {
+        put(c);
+        use();
+      }
+  }
+  if (tail && nfull % NW == wave) {
+    // what whole blocks leave over: the row's last block, without the elements that were summed already; rows shorter than a block: one by one
+    const long skip = (p.kk - BLK) * (long)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < NL; ++i)
+      if (i < NWL || i - NWL < xgroups)
+        v[0][i] = nfull ? lin_keep_from<T>(*reinterpret_cast<const lin_u4_any*>(src(i) + skip + off[i]), BLK - tail - piece * EL)
+                        : lin_load_first<T>(reinterpret_cast<const T*>(src(i) + (off[i] - piece * 16)), reinterpret_cast<const T*>(src(i) + off[i]),
+                                            tail - piece * EL);
+    put(0);
+    use();
+  }
+  __syncthreads();                                    // every wave is done with its stage: the sums take the same LDS
+  float(*red)[G][MT][256] = reinterpret_cast<float(*)[G][MT][256]>(lds);
   // D register r: weight row 4 (lane >> 4) + r, x row lane & 15
 #pragma unroll
   for (int g = 0; g < G; ++g)
