@@ -11,7 +11,7 @@ from tracknetv3_amd import _lib, feedforward as ff, ops
 
 @pytest.mark.parametrize("dtype", lc.DTYPES)
 @pytest.mark.parametrize("gated", [False, True])
-@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 64, 32), (3, 5, 7), (17, 72, 40), (33, 129, 65), (5, 200, 20), (66, 70, 33), (130, 40, 136)])
+@pytest.mark.parametrize("rows,k,n", [(1, 1, 1), (1, 64, 32), (3, 5, 7), (17, 72, 40), (33, 129, 65), (5, 200, 20), (66, 70, 33), (67, 33, 66), (130, 40, 136)])
 def test_exact_integers(emu, rows, k, n, gated, dtype):
     lc.check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device="cpu", seed=rows + k)
 
@@ -50,6 +50,7 @@ def test_direct_loads_land_before_they_are_read(emu, monkeypatch, cus, lazy):
     for dtype in lc.DTYPES:
         lc.check_exact(70, 200, 264, dtype, False, True, True, "cpu")
         lc.check_exact(130, 264, 136, dtype, True, True, False, "cpu")
+        lc.check_exact(75, 131, 69, dtype, True, True, False, "cpu")
 
 
 @pytest.mark.parametrize("cus", ["1", "256"])
@@ -171,3 +172,7 @@ def test_refusals(emu):
     assert lib.tnv3_linear_forward(*args, p(ws), long_k - 4, 70, 1100, 24, 0, 0, null) != 0                                  # too small
     assert lib.tnv3_linear_forward(*args, p(ws), long_k, 70, 1100, 24, 0, 0, null) == 0
     assert lib.tnv3_linear_forward_workspace_bytes(0, 1, 1, 0) == 0
+    off = torch.zeros(4 * 8 + 1)[1:].view(4, 8)                                                                              # 4 bytes off the boundary
+    assert fwd(xp=p(off)) != 0 and fwd() == 0
+    assert torch.equal(ops.linear(off + 1, torch.ones(6, 8)), torch.full((4, 6), 8.0))
+    assert torch.equal(ops.linear(off, w), torch.zeros(4, 6))                                                                # the op copies such a view

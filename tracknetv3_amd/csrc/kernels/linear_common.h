@@ -197,6 +197,24 @@ template <bool FAST> __device__ __forceinline__ void lin_act8(float (&v)[8], int
 #undef TNV3_LIN_ACT_CASE
 }
 
+// ---- LDS tiles
+// Position (in 16-bit elements) of 8-element chunk c of row r in an LDS tile.  k-contiguous rows of BK elements: rows 8 apart would share
+// their banks, so the chunk index is exchanged with row bits -- a fragment read's eight lanes then cover all banks once.  k-strided tiles are rows of `ld`
+// elements; the transposing read takes 4 rows x 32 bytes at a time: row bits move the 32-byte piece.
+template <int BK> __device__ __forceinline__ int lin_pos_kc(int r, int c) { return r * BK + ((c ^ (BK == 64 ? (r & 7) : ((r >> 1) & 3))) << 3); }
+__device__ __forceinline__ int lin_pos_ks(int k, int c, int ld) { return k * ld + ((c ^ ((k & 3) << 1)) << 3); }
+
+// fragments of one operand: rows base + 32 t + (l & 31), k = 16 s + 8 (l >> 5) + 0..7
+template <bool KS, int BK, int ROWS>
+__device__ __forceinline__ lin_s8 lin_frag(const unsigned short* tile, int base, int t, int s, int lane) {
+  if (!KS) return *reinterpret_cast<const lin_s8*>(tile + lin_pos_kc<BK>(base + 32 * t + (lane & 31), 2 * s + (lane >> 5)));
+  const int q = lane & 15, c = ((base + 32 * t) >> 3) + ((lane >> 4) & 1) * 2 + ((q & 3) >> 1);
+  const int k = 16 * s + 8 * (lane >> 5) + (q >> 2);
+  const unsigned short* p = tile + lin_pos_ks(k, c, ROWS) + (q & 1) * 4;
+  const lin_s4 lo = lin_lds_tr4(p), hi = lin_lds_tr4(p + 4 * ROWS);
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // ---- one product's arguments
 struct LinGemmArgs {
   const void* a;          // element (i, k) at a[i * lda + k], or a[k * lda + i] where the kernel's operand is strided in k
@@ -213,16 +231,16 @@ struct LinGemmArgs {
   int f;                  // gated: F
   int tiles_i, tiles_j, splits;
   long k_per_split;       // a multiple of the kernel's k step
-  int vec;                // bit 0 / 1: a / b can be read in whole 16-byte pieces; bit 2: the outputs (and bias, residual) are such
+  bool vec;               // the outputs' rows (bias, residual) are whole 16-byte pieces
 };
-enum { kLinVecA = 1, kLinVecB = 2, kLinVecOut = 4 };
 
-// blockIdx -> (tile_i, tile_j, split).  Workgroups go to the 8 XCDs in turn, and each XCD has its own L2: XCD x gets the x-th contiguous
+// block -> (tile_i, tile_j, split); false: beyond the last.  Workgroups go to the 8 XCDs in turn, and each XCD has its own L2: XCD x gets the x-th contiguous
 // eighth of the tile list, and the list walks 8 tiles of i within a panel before the next j, so that the ~32 tiles an XCD works on at a time
 // share 8 panels of A and 4 of B.
-__device__ __forceinline__ void lin_tile(const LinGemmArgs& p, int& ti, int& tj, int& sp) {
+__device__ __forceinline__ bool lin_tile(const LinGemmArgs& p, int b, int& ti, int& tj, int& sp) {
   const int tiles = p.tiles_i * p.tiles_j, total = tiles * p.splits;
-  const int b = blockIdx.x, per = total >> 3, rem = total & 7, x = b & 7;
+  if (b >= total) return false;
+  const int per = total >> 3, rem = total & 7, x = b & 7;
   int t = x * per + (x < rem ? x : rem) + (b >> 3);
   sp = t / tiles;
   t -= sp * tiles;
@@ -230,6 +248,7 @@ __device__ __forceinline__ void lin_tile(const LinGemmArgs& p, int& ti, int& tj,
   const int left = p.tiles_i - 8 * g, gh = left < 8 ? left : 8;
   tj = in / gh;
   ti = 8 * g + (in - tj * gh);
+  return true;
 }
 
 // ---- write-out of eight consecutive columns of one row; v: fp32 sums (gated: v gate, u the other factor)
@@ -237,7 +256,7 @@ template <class T>
 __device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j, float (&v)[8], const float (&bias)[8]) {
   if (i >= p.rows_i || j >= p.rows_j) return;
   const int n = p.rows_j - j < 8 ? (int)(p.rows_j - j) : 8;
-  const bool vec = (p.vec & kLinVecOut) && n == 8;
+  const bool vec = p.vec && n == 8;
   const long o = i * p.rows_j + j;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
@@ -256,7 +275,7 @@ __device__ __forceinline__ void lin_finish_gated8(const LinGemmArgs& p, long i, 
                                                   const float (&bu)[8]) {
   if (i >= p.rows_i || j >= p.f) return;
   const int n = p.f - j < 8 ? (int)(p.f - j) : 8;
-  const bool vec = (p.vec & kLinVecOut) && n == 8;
+  const bool vec = p.vec && n == 8;
 #pragma unroll
   for (int e = 0; e < 8; ++e) { g[e] += bg[e]; u[e] += bu[e]; }
   if (p.pre) {
@@ -273,7 +292,7 @@ template <class T>
 __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&b)[8]) {
   const long left = p.rows_j - j;
   const int n = left < 8 ? (left < 0 ? 0 : (int)left) : 8;
-  if (p.bias) lin_load8<T>(static_cast<const T*>(p.bias) + (n > 0 ? j : 0), b, (p.vec & kLinVecOut) && n == 8, n);
+  if (p.bias) lin_load8<T>(static_cast<const T*>(p.bias) + (n > 0 ? j : 0), b, p.vec && n == 8, n);
   else
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[e] = 0.0f;
@@ -323,7 +342,7 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16
             float* part = p.part + ((long)sp * p.rows_i + i) * p.rows_j;
             const long lim = GATED ? p.f : p.rows_j;
             const int n = lim - j < 8 ? (int)(lim - j) : 8;
-            const bool vec = (p.vec & kLinVecOut) && n == 8;
+            const bool vec = p.vec && n == 8;
             lin_store8<float>(part + j, v, vec, n);
             if (GATED) lin_store8<float>(part + p.f + j, u, vec, n);
           }
@@ -339,13 +358,13 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16
 
 // ---- joins the partial sums of a split contraction in a fixed order and finishes them: one work-item per 8 columns of a row
 template <class T, bool GATED>
-__global__ void __launch_bounds__(256) lin_join_kernel(const LinGemmArgs p) {
+__device__ __forceinline__ void lin_join(const LinGemmArgs& p, long block) {
   const long cols = GATED ? p.f : p.rows_j, pieces = (cols + 7) / 8;
-  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  const long t = block * 256 + threadIdx.x;
   const long i = t / pieces, j = (t - i * pieces) * 8;
   if (i >= p.rows_i) return;
   const int n = cols - j < 8 ? (int)(cols - j) : 8;
-  const bool vec = (p.vec & kLinVecOut) && n == 8;
+  const bool vec = p.vec && n == 8;
   float v[8], u[8], q[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.0f;
@@ -368,6 +387,71 @@ __global__ void __launch_bounds__(256) lin_join_kernel(const LinGemmArgs p) {
   } else {
     lin_finish8<T>(p, i, j, v, b0);
   }
+}
+
+template <class T, bool GATED>
+__global__ void __launch_bounds__(256) lin_join_kernel(const LinGemmArgs p) { lin_join<T, GATED>(p, blockIdx.x); }
+
+// ---- a backward pass's products in one launch: blocks [0, blocks_dx) the gradient of x, then blocks_dw the gradient of W, then the bias gradient's
+// column sums from their row blocks' partial sums; a count of 0 leaves one out.  The first two counts are multiples of 8 (XCDs).
+struct LinPairArgs {
+  LinGemmArgs dx, dw;
+  const float* sums;      // [sum_rows][sum_cols]
+  void* db;
+  int blocks_dx, blocks_dw, sum_rows, sum_cols;
+};
+// 128 columns per workgroup, NT / 128 work-items per column, joined in order
+template <class T, int NT>
+__device__ __forceinline__ void lin_colsum(const float* __restrict__ part, T* __restrict__ out, int rows, int cols, int block, float* red) {
+  constexpr int Y = NT / 128;
+  const int c = threadIdx.x & 127, y = threadIdx.x >> 7, j = block * 128 + c;
+  float s = 0.0f;
+  if (j < cols) {
+#pragma unroll 8
+    for (int r = y; r < rows; r += Y) s += part[(long)r * cols + j];
+  }
+  red[threadIdx.x] = s;
+  __syncthreads();
+  if (y || j >= cols) return;
+#pragma unroll
+  for (int q = 1; q < Y; ++q) s += red[q * 128 + c];
+  lin_down(s, out[j]);
+}
+template <class T>
+__global__ void __launch_bounds__(256) lin_join_pair_kernel(const LinPairArgs p) {
+  // blocks_dx / blocks_dw: of this launch
+  if ((int)blockIdx.x < p.blocks_dx) lin_join<T, false>(p.dx, blockIdx.x);
+  else lin_join<T, false>(p.dw, (long)blockIdx.x - p.blocks_dx);
+}
+
+// ---- 16-bit operands whose rows are no whole 16-byte pieces: copied once into rows that are, the added columns 0.  Bound by memory (each element
+// read and written once); the products then take the direct loads at full speed.
+struct LinPadArgs {
+  const unsigned short* src[2];
+  unsigned short* dst[2];
+  long rows[2];
+  int width[2];
+  long blocks0;           // workgroups of the first of the two
+};
+inline __host__ __device__ int lin_pad_width(int w) { return (w + 7) / 8 * 8; }
+inline __global__ void __launch_bounds__(256) lin_pad_kernel(const LinPadArgs p) {
+  const int o = (long)blockIdx.x >= p.blocks0;
+  const long t = ((long)blockIdx.x - (o ? p.blocks0 : 0)) * 256 + threadIdx.x;
+  const int w = p.width[o], pieces = (w + 7) / 8;
+  const long r = t / pieces;
+  const int c = (int)(t - r * pieces) * 8;
+  if (r >= p.rows[o]) return;
+  typedef unsigned u4_any __attribute__((ext_vector_type(4), aligned(2)));
+  const unsigned short* s = p.src[o] + r * w + c;
+  lin_u4 q = {0u, 0u, 0u, 0u};
+  if (c + 8 <= w) {
+    q = *reinterpret_cast<const u4_any*>(s);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < w) q[e >> 1] |= (unsigned)s[e] << (16 * (e & 1));
+  }
+  *reinterpret_cast<lin_u4*>(p.dst[o] + (r * pieces) * 8 + c) = q;
 }
 
 }  // namespace tnv3

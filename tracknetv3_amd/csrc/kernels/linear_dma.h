@@ -7,7 +7,6 @@
 // quarter step (8 or 4 MFMAs of 32 cycles per wave, two waves per SIMD) earlier.
 #pragma once
 #include "linear_common.h"
-#include "linear_staged.h"
 
 namespace tnv3 {
 
@@ -70,13 +69,12 @@ __device__ __forceinline__ void lin_dma_sync() {
 }
 
 template <class Cfg, class T, bool KSA, bool KSB, bool GATED>
-__global__ void __launch_bounds__(Cfg::NT, 2) lin_dma_kernel(const LinGemmArgs p) {
+__device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block, unsigned short* lds) {
   constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, STAGE = Cfg::STAGE, Q = BK / 16;
-  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / Cfg::WN, wj = wave % Cfg::WN;
   int ti, tj, sp;
-  lin_tile(p, ti, tj, sp);
+  if (!lin_tile(p, block, ti, tj, sp)) return;
   const long i0 = (long)ti * BI, j0 = (long)tj * (GATED ? BJ / 2 : BJ);
   const long kbeg = (long)sp * p.k_per_split, kend = kbeg + p.k_per_split < p.kk ? kbeg + p.k_per_split : p.kk;
   const int steps = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
@@ -151,6 +149,20 @@ __global__ void __launch_bounds__(Cfg::NT, 2) lin_dma_kernel(const LinGemmArgs p
   lin_dma_sync();
   lin_write_out<T, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                   j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
+}
+
+template <class Cfg, class T, bool GATED>
+__global__ void __launch_bounds__(Cfg::NT, 2) lin_dma_kernel(const LinGemmArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
+  lin_dma_product<Cfg, T, false, false, GATED>(p, blockIdx.x, lds);
+}
+template <class Cfg, class T>
+__global__ void __launch_bounds__(Cfg::NT, 2) lin_dma_pair_kernel(const LinPairArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
+  const int b = blockIdx.x, c = b - p.blocks_dx, d = c - p.blocks_dw;
+  if (c < 0) lin_dma_product<Cfg, T, false, true, false>(p.dx, b, lds);
+  else if (d < 0) lin_dma_product<Cfg, T, true, true, false>(p.dw, c, lds);
+  else lin_colsum<T, Cfg::NT>(p.sums, static_cast<T*>(p.db), p.sum_rows, p.sum_cols, d, reinterpret_cast<float*>(lds));
 }
 
 }  // namespace tnv3

@@ -4,7 +4,7 @@
 // exact ones behind a chain of layers (measured: 3.4e-3 of the weight gradient's norm in bf16, a single rounding being 1.7e-3).
 // And the bias gradient, the column sums of dz.  Bound by memory: dy and z are read and dz is written once, in 16-byte pieces.  A workgroup takes 256
 // columns (32 work-items of 8) and every 8th row of its row block per work-item; its column sums are joined through LDS and written as
-// partial sums [row block][columns], which lin_colsum_kernel adds in order: no atomics, the same bits from run to run.
+// partial sums [row block][columns], which lin_colsum adds in order: no atomics, the same bits from run to run.
 #pragma once
 #include "linear_common.h"
 
@@ -13,7 +13,8 @@ namespace tnv3 {
 struct LinDzArgs {
   const void* dy;        // [rows][n]
   const void* pre;       // [rows][n], gated [rows][2 n] in fp32; null: no activation, only the column sums are wanted
-  void* dz;              // [rows][n] / [rows][2 n]; null with pre
+  void* dz;              // [rows][ld_dz] of which n / 2 n columns hold dz and the others become 0; null with pre
+  int ld_dz;
   float* part;           // [row blocks][n] / [..][2 n], or null: no bias
   long rows;
   int n, act, rows_per_block, vec;
@@ -38,7 +39,7 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(const LinDzArgs p) {
       float d[8], g[8], u[8];
       lin_load8<T>(static_cast<const T*>(p.dy) + r * p.n + j, d, vec, n);
       if (p.pre) {
-        T* o = static_cast<T*>(p.dz) + r * ldz + j;
+        T* o = static_cast<T*>(p.dz) + r * p.ld_dz + j;
         if (GATED) {
           const float* z = static_cast<const float*>(p.pre) + r * ldz + j;
           lin_load8<float>(z, g, vec, n);
@@ -65,6 +66,10 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(const LinDzArgs p) {
 #undef TNV3_LIN_DZ_CASE
         lin_store8<T>(o, g, vec, n);
         if (GATED) lin_store8<T>(o + p.n, u, vec, n);
+        if (j + 8 >= p.n) {                                // the last columns' work-item clears what the row is padded with
+          T* end = static_cast<T*>(p.dz) + r * p.ld_dz;
+          for (int c = ldz; c < p.ld_dz; ++c) end[c] = T{};
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) { s0[e] += g[e]; if (GATED) s1[e] += u[e]; }
       } else {
@@ -89,16 +94,6 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(const LinDzArgs p) {
     for (int y = 0; y < 8; ++y) s += red[h][y][c];
     p.part[rb * ldz + h * p.n + col] = s;
   }
-}
-
-// out[j] = sum over the row blocks, in order
-template <class T>
-__global__ void __launch_bounds__(256) lin_colsum_kernel(const float* __restrict__ part, T* __restrict__ out, int n, int blocks) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= n) return;
-  float s = 0.0f;
-  for (int b = 0; b < blocks; ++b) s += part[(long)b * n + j];
-  lin_down(s, out[j]);
 }
 
 }  // namespace tnv3

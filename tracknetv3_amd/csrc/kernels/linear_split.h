@@ -16,7 +16,6 @@
 // half's fragments are in registers by then, the next step's first fragments are read under the second half's products.
 #pragma once
 #include "linear_common.h"
-#include "linear_staged.h"
 
 namespace tnv3 {
 
@@ -104,15 +103,13 @@ struct LinSplitLoader {
 };
 
 template <class Cfg, bool KSA, bool KSB, bool GATED>
-__global__ void __launch_bounds__(Cfg::NT, 2) lin_split_kernel(const LinGemmArgs p) {
+__device__ __forceinline__ void lin_split_product(const LinGemmArgs& p, int block, unsigned short* lds, int& redo) {
   constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, NT = Cfg::NT, STAGE = Cfg::STAGE;
   constexpr int A_PLANE = Cfg::A_PLANE, B_PLANE = Cfg::B_PLANE;
-  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
-  __shared__ int redo;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / Cfg::WN, wj = wave % Cfg::WN;
   int ti, tj, sp;
-  lin_tile(p, ti, tj, sp);
+  if (!lin_tile(p, block, ti, tj, sp)) return;
   const long i0 = (long)ti * BI, j0 = (long)tj * (GATED ? BJ / 2 : BJ);
   const long kbeg = (long)sp * p.k_per_split, kend = kbeg + p.k_per_split < p.kk ? kbeg + p.k_per_split : p.kk;
   const int steps = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
@@ -253,6 +250,22 @@ __global__ void __launch_bounds__(Cfg::NT, 2) lin_split_kernel(const LinGemmArgs
   }
   lin_write_out<float, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                       j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
+}
+
+template <class Cfg, bool GATED>
+__global__ void __launch_bounds__(Cfg::NT, 2) lin_split_kernel(const LinGemmArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
+  __shared__ int redo;
+  lin_split_product<Cfg, false, false, GATED>(p, blockIdx.x, lds, redo);
+}
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::NT, 2) lin_split_pair_kernel(const LinPairArgs p) {
+  __shared__ __attribute__((aligned(1024))) unsigned short lds[Cfg::LDS];
+  __shared__ int redo;
+  const int b = blockIdx.x, c = b - p.blocks_dx, d = c - p.blocks_dw;
+  if (c < 0) lin_split_product<Cfg, false, true, false>(p.dx, b, lds, redo);
+  else if (d < 0) lin_split_product<Cfg, true, true, false>(p.dw, c, lds, redo);
+  else lin_colsum<float, Cfg::NT>(p.sums, static_cast<float*>(p.db), p.sum_rows, p.sum_cols, d, reinterpret_cast<float*>(lds));
 }
 
 }  // namespace tnv3

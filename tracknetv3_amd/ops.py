@@ -1216,6 +1216,11 @@ def _address(t):
     return None if t is None else t.data_ptr()
 
 
+def _boundary(t):
+    """t, or its copy if it is a view that starts off a 16-byte boundary."""
+    return t if t is None or not t.data_ptr() & 15 else t.clone()
+
+
 def _linear_stream(x):
     return torch._C._cuda_getCurrentRawStream(x.get_device()) if x.is_cuda else 0
 
@@ -1231,6 +1236,7 @@ def linear(x, weight, bias=None, residual=None, act=ACT_NONE, want_pre=False):
     y = torch.empty(shape, dtype=x.dtype, device=x.device)
     pre = torch.empty_like(y) if want_pre and act != ACT_NONE else None
     if rows:
+        x, weight, bias, residual = _boundary(x), _boundary(weight), _boundary(bias), _boundary(residual)
         ws, need = _linear_workspace(lib, "tnv3_linear_forward_workspace_bytes", x, rows, k, n, code)
         _lib.check(lib.tnv3_linear_forward(x.data_ptr(), weight.data_ptr(), _address(bias), _address(residual), y.data_ptr(), _address(pre), _address(ws),
                                            need, rows, k, n, act, code, _linear_stream(x)))
@@ -1245,6 +1251,7 @@ def gated_linear(x, weight, bias=None, act=ACT_SILU, want_pre=False):
     h = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
     pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=torch.float32, device=x.device) if want_pre else None
     if rows:
+        x, weight, bias = _boundary(x), _boundary(weight), _boundary(bias)
         ws, need = _linear_workspace(lib, "tnv3_gated_linear_forward_workspace_bytes", x, rows, k, n, code)
         _lib.check(lib.tnv3_gated_linear_forward(x.data_ptr(), weight.data_ptr(), _address(bias), h.data_ptr(), _address(pre), _address(ws), need, rows,
                                                  k, n, act, code, _linear_stream(x)))
@@ -1269,6 +1276,7 @@ def _linear_backward_call(gated, dy, x, weight, pre, act, want, rows, k, n, code
     if rows == 0:
         return (torch.empty_like(x) if want[0] else None, torch.zeros_like(weight) if want[1] else None,
                 torch.zeros(n2, dtype=x.dtype, device=x.device) if want[2] else None)
+    dy, x, weight, pre = _boundary(dy), _boundary(x), _boundary(weight), _boundary(pre)
     dx = torch.empty_like(x) if want[0] else None
     dw = torch.empty_like(weight) if want[1] else None
     db = torch.empty(n2, dtype=x.dtype, device=x.device) if want[2] else None
