@@ -198,11 +198,12 @@ template <bool FAST> __device__ __forceinline__ void lin_act8(float (&v)[8], int
 }
 
 // ---- LDS tiles
-// Position (in 16-bit elements) of 8-element chunk c of row r in an LDS tile.  k-contiguous rows of BK elements: rows 8 apart would share
-// their banks, so the chunk index is exchanged with row bits -- a fragment read's eight lanes then cover all banks once.  k-strided tiles are rows of `ld`
-// elements; the transposing read takes 4 rows x 32 bytes at a time: row bits move the 32-byte piece.
-template <int BK> __device__ __forceinline__ int lin_pos_kc(int r, int c) { return r * BK + ((c ^ (BK == 64 ? (r & 7) : ((r >> 1) & 3))) << 3); }
-__device__ __forceinline__ int lin_pos_ks(int k, int c, int ld) { return k * ld + ((c ^ ((k & 3) << 1)) << 3); }
+// Position (in 16-bit elements) of 8-element chunk c of row r in an LDS tile.  LDS has 64 banks of 4 bytes: a 16-byte fragment read serves 16 lanes
+// (16 rows of one chunk) per clock if they name 16 different 16-byte slots of 256 bytes, the transposing read 32 lanes (4 rows of k, two 32-byte
+// pieces each).  So the chunk index is exchanged with those row bits that rows of this length leave out of the bank number.  (With 32 banks' worth of row
+// bits half of all LDS cycles were conflicts.)
+template <int BK> __device__ __forceinline__ int lin_pos_kc(int r, int c) { return r * BK + ((c ^ (BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3)) << 3); }
+__device__ __forceinline__ int lin_pos_ks(int k, int c, int ld) { return k * ld + ((c ^ (ld == 64 ? (k & 2) << 1 : (k & 3) << 2)) << 3); }
 
 // fragments of one operand: rows base + 32 t + (l & 31), k = 16 s + 8 (l >> 5) + 0..7
 template <bool KS, int BK, int ROWS>

@@ -26,7 +26,7 @@ struct LinDma {
   static constexpr int N = ROWS / 8 / NW;
   static_assert(N * 8 * NW == ROWS, "whole pieces per wave");
   unsigned off[N];          // bytes from the operand's first element of the step
-  int kchunk;               // k-contiguous: first k of the lane's chunk
+  int kchunk;               // k-contiguous: first k of the lane's chunk in its even pieces
   const char* base;
   long left;                // bytes from base to the operand's end
   long step;                // bytes per step
@@ -40,12 +40,14 @@ struct LinDma {
       const int piece = wave * N + i;
       if (KS) {
         constexpr int LPR = ROWS / 8;
-        const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((k & 3) << 1);
+        static_assert(ROWS >= 128, "lin_pos_ks's order for these rows");
+        const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((k & 3) << 2);
         off[i] = (unsigned)(k * (int)(2 * ld) + c * 16);
       } else {
-        const int r = lane >> 3, c = (lane & 7) ^ r;
+        static_assert(N % 2 == 0, "piece i of a wave is odd where i is");
+        const int r = lane >> 3, c = (lane & 7) ^ (r >> 1) ^ ((i & 1) << 2);            // lin_pos_kc's order
         off[i] = (unsigned)((piece * 8 + r) * (int)(2 * ld) + c * 16);
-        kchunk = c * 8;
+        if (i == 0) kchunk = c * 8;
       }
     }
   }
@@ -55,7 +57,7 @@ struct LinDma {
     const tnv3_rsrc_t r = tnv3_make_rsrc(base, bytes);
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      tnv3_buf_dma16(r, reinterpret_cast<float*>(tile + (wave * N + i) * 512), !KS && kchunk >= kleft ? kDmaOob : off[i]);
+      tnv3_buf_dma16(r, reinterpret_cast<float*>(tile + (wave * N + i) * 512), !KS && (kchunk ^ ((i & 1) << 5)) >= kleft ? kDmaOob : off[i]);
     base += step;
     left -= step;
   }
