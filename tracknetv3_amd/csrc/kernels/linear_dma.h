@@ -51,15 +51,17 @@ struct LinDma {
       }
     }
   }
-  // kleft: elements of the contraction left in this split from the step's first on
-  __device__ __forceinline__ void issue(unsigned short* tile, long kleft, int wave) {
+  // the step's descriptor; then the next step's base
+  __device__ __forceinline__ tnv3_rsrc_t begin() {
     const unsigned bytes = left <= 0 ? 0u : (left > 0x7fffffffl ? 0x7fffffffu : (unsigned)left);
     const tnv3_rsrc_t r = tnv3_make_rsrc(base, bytes);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      tnv3_buf_dma16(r, reinterpret_cast<float*>(tile + (wave * N + i) * 512), !KS && (kchunk ^ ((i & 1) << 5)) >= kleft ? kDmaOob : off[i]);
     base += step;
     left -= step;
+    return r;
+  }
+  // piece i; kleft: elements of the contraction left in this split from the step's first on (none: zeros arrive)
+  __device__ __forceinline__ void piece(tnv3_rsrc_t r, unsigned short* tile, int i, int kleft, int wave) {
+    tnv3_buf_dma16(r, reinterpret_cast<float*>(tile + (wave * N + i) * 512), (KS ? 0 : kchunk ^ ((i & 1) << 5)) >= kleft ? kDmaOob : off[i]);
   }
 };
 
@@ -95,12 +97,23 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
   } else {
     db.init(p.b, KSB ? kbeg * p.ldb + j0 : j0 * p.ldb + kbeg, KSB ? p.kk * p.ldb : p.rows_j * p.ldb, p.ldb, wave, lane);
   }
+  // the stage being filled: its descriptors, its place, what is left of the contraction there
   long kleft = kend - kbeg;
-  auto dma = [&](int s) {
-    unsigned short* t = lds + (s & 1) * STAGE;
-    da.issue(t, kleft, wave);
-    db.issue(t + BI * BK, kleft, wave);
+  tnv3_rsrc_t ra, rb;
+  unsigned short* into = lds;
+  int kl = 0;
+  auto begin = [&](int s) {
+    ra = da.begin();
+    rb = db.begin();
+    into = lds + (s & 1) * STAGE;
+    kl = kleft > BK ? BK : (kleft > 0 ? (int)kleft : 0);
     kleft -= BK;
+  };
+  constexpr int NA = LinDma<KSA, BI, Cfg::NW>::N, NP = NA + LinDma<KSB, BJ, Cfg::NW>::N;
+  auto piece = [&](int i) {
+    if (i >= NP) return;
+    if (i < NA) da.piece(ra, into, i, kl, wave);
+    else db.piece(rb, into + BI * BK, i - NA, kl, wave);
   };
 
   f32x16 acc[TM][TN];
@@ -119,19 +132,35 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
 #pragma unroll
     for (int y = 0; y < TN; ++y) fb[set][y] = lin_frag<KSB, BK, BJ>(t + BI * BK, wj * TN * 32, y, q, lane);
   };
-  auto products = [&](int set) {
+  // the products of one quarter, PQ pieces of direct loads (first .. first + PQ - 1) between them: a wave's loads queue behind those of the CU's other
+  // waves (16 clocks of the address path each), so they are spread over three quarters instead of standing in front of the products
+  constexpr int PQ = 3, GAP = TM * TN / (PQ + 1) > 0 ? TM * TN / (PQ + 1) : 1;
+  auto products = [&](int set, int first) {
 #pragma unroll
     for (int y = 0; y < TN; ++y)
 #pragma unroll
-      for (int x = 0; x < TM; ++x) acc[x][y] = lin_mfma(fa[set][x], fb[set][y], acc[x][y], T{});
+      for (int x = 0; x < TM; ++x) {
+        const int m = y * TM + x;
+        acc[x][y] = lin_mfma(fa[set][x], fb[set][y], acc[x][y], T{});
+        if (first >= 0 && m % GAP == GAP - 1 && m / GAP < PQ) {
+          __builtin_amdgcn_sched_barrier(0);
+          piece(first + m / GAP);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
   };
 
   if (steps > 0) {
-    dma(0);
+    begin(0);
+#pragma unroll
+    for (int i = 0; i < NP; ++i) piece(i);
     lin_dma_sync();
-    if (steps > 1) dma(1);
+    begin(1);
+#pragma unroll
+    for (int i = 0; i < PQ; ++i) piece(i);
     read(0, 0, 0);
   }
+  static_assert(Q == 4 && NP <= 3 * PQ, "a stage's pieces: the last quarter of the step before, the first two of the step");
   for (int s = 0; s < steps; ++s) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -139,12 +168,12 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
         read(s, q + 1, (q + 1) & 1);
       } else {
         lin_dma_sync();
-        if (s + 2 < steps) dma(s + 2);
-        if (s + 1 < steps) read(s + 1, 0, 0);
+        begin(s + 2);                         // (beyond the last step: zeros into a stage that is not read)
+        read(s + 1, 0, 0);
       }
       // (the fences keep the reads ahead of the products: left alone, the scheduler puts each read right in front of its use)
       __builtin_amdgcn_sched_barrier(0);
-      products(q & 1);
+      products(q & 1, q == 3 ? 0 : (q == 0 ? PQ : (q == 1 ? 2 * PQ : -1)));
       __builtin_amdgcn_sched_barrier(0);
     }
   }
