@@ -133,8 +133,8 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     for (int y = 0; y < TN; ++y) fb[set][y] = lin_frag<KSB, BK, BJ>(t + BI * BK, wj * TN * 32, y, q, lane);
   };
   // the products of one quarter, PQ pieces of direct loads (first .. first + PQ - 1) between them: a wave's loads queue behind those of the CU's other
-  // waves (16 clocks of the address path each), so they are spread over three quarters instead of standing in front of the products
-  constexpr int PQ = 3, GAP = TM * TN / (PQ + 1) > 0 ? TM * TN / (PQ + 1) : 1;
+  // waves (16 clocks of the address path each), so they are spread over two quarters instead of standing in front of the products
+  constexpr int PQ = 4, GAP = TM * TN / PQ;
   auto products = [&](int set, int first) {
 #pragma unroll
     for (int y = 0; y < TN; ++y)
@@ -160,7 +160,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     for (int i = 0; i < PQ; ++i) piece(i);
     read(0, 0, 0);
   }
-  static_assert(Q == 4 && NP <= 3 * PQ, "a stage's pieces: the last quarter of the step before, the first two of the step");
+  static_assert(Q == 4 && NP <= 2 * PQ && GAP > 0, "a stage's pieces: the last quarter of the step before, the first of the step");
   for (int s = 0; s < steps; ++s) {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -173,7 +173,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       }
       // (the fences keep the reads ahead of the products: left alone, the scheduler puts each read right in front of its use)
       __builtin_amdgcn_sched_barrier(0);
-      products(q & 1, q == 3 ? 0 : (q == 0 ? PQ : (q == 1 ? 2 * PQ : -1)));
+      products(q & 1, q == 3 ? 0 : (q == 0 ? PQ : -1));
       __builtin_amdgcn_sched_barrier(0);
     }
   }
