@@ -97,20 +97,18 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
   } else {
     db.init(p.b, KSB ? kbeg * p.ldb + j0 : j0 * p.ldb + kbeg, KSB ? p.kk * p.ldb : p.rows_j * p.ldb, p.ldb, wave, lane);
   }
-  // the stage being filled: its descriptors, its place, what is left of the contraction there
+  // the stage being filled: its descriptors, what is left of the contraction there
   long kleft = kend - kbeg;
   tnv3_rsrc_t ra, rb;
-  unsigned short* into = lds;
   int kl = 0;
-  auto begin = [&](int s) {
+  auto begin = [&]() {
     ra = da.begin();
     rb = db.begin();
-    into = lds + (s & 1) * STAGE;
     kl = kleft > BK ? BK : (kleft > 0 ? (int)kleft : 0);
     kleft -= BK;
   };
   constexpr int NA = LinDma<KSA, BI, Cfg::NW>::N, NP = NA + LinDma<KSB, BJ, Cfg::NW>::N;
-  auto piece = [&](int i) {
+  auto piece = [&](unsigned short* into, int i) {
     if (i >= NP) return;
     if (i < NA) da.piece(ra, into, i, kl, wave);
     else db.piece(rb, into + BI * BK, i - NA, kl, wave);
@@ -125,8 +123,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
 
   lin_s8 fa[2][TM], fb[2][TN];
-  auto read = [&](int s, int q, int set) {
-    const unsigned short* t = lds + (s & 1) * STAGE;
+  auto read = [&](const unsigned short* t, int q, int set) {
 #pragma unroll
     for (int x = 0; x < TM; ++x) fa[set][x] = lin_frag<KSA, BK, BI>(t, wi * TM * 32, x, q, lane);
 #pragma unroll
@@ -135,7 +132,8 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
   // the products of one quarter, PQ pieces of direct loads (first .. first + PQ - 1) between them: a wave's loads queue behind those of the CU's other
   // waves (16 clocks of the address path each), so they are spread over two quarters instead of standing in front of the products
   constexpr int PQ = 4, GAP = TM * TN / PQ;
-  auto products = [&](int set, int first) {
+  static_assert(Q == 4 && NP <= 2 * PQ && GAP > 0, "a stage's pieces: two quarters");
+  auto products = [&](int set, unsigned short* into, int first) {
 #pragma unroll
     for (int y = 0; y < TN; ++y)
 #pragma unroll
@@ -144,40 +142,43 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
         acc[x][y] = lin_mfma(fa[set][x], fb[set][y], acc[x][y], T{});
         if (first >= 0 && m % GAP == GAP - 1 && m / GAP < PQ) {
           __builtin_amdgcn_sched_barrier(0);
-          piece(first + m / GAP);
+          piece(into, first + m / GAP);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
   };
-
-  if (steps > 0) {
-    begin(0);
+  // From one barrier to the next: the last quarter's products of the step before (its fragments are in registers), then three quarters of this one.
+  // Every read is from `rd`, every direct load goes to `wr`, the other stage.  (The qualifiers say so to the compiler, which otherwise lets each
+  // transposing read wait for all loads in flight.  The fences keep the reads ahead of the products: left alone, the scheduler puts each read right
+  // in front of its use.)
+  auto step = [&](const unsigned short* __restrict__ rd, unsigned short* __restrict__ wr, auto first) {
+    begin();                                    // (beyond the last step: zeros into a stage that is not read)
+    read(rd, 0, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (decltype(first)::value) {
 #pragma unroll
-    for (int i = 0; i < NP; ++i) piece(i);
-    lin_dma_sync();
-    begin(1);
-#pragma unroll
-    for (int i = 0; i < PQ; ++i) piece(i);
-    read(0, 0, 0);
-  }
-  static_assert(Q == 4 && NP <= 2 * PQ && GAP > 0, "a stage's pieces: the last quarter of the step before, the first of the step");
-  for (int s = 0; s < steps; ++s) {
-#pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      if (q + 1 < Q) {
-        read(s, q + 1, (q + 1) & 1);
-      } else {
-        lin_dma_sync();
-        begin(s + 2);                         // (beyond the last step: zeros into a stage that is not read)
-        read(s + 1, 0, 0);
-      }
-      // (the fences keep the reads ahead of the products: left alone, the scheduler puts each read right in front of its use)
-      __builtin_amdgcn_sched_barrier(0);
-      products(q & 1, q == 3 ? 0 : (q == 0 ? PQ : -1));
-      __builtin_amdgcn_sched_barrier(0);
+      for (int i = 0; i < PQ; ++i) piece(wr, i);
+    } else {
+      products(1, wr, 0);
     }
+#pragma unroll
+    for (int q = 0; q + 1 < Q; ++q) {
+      __builtin_amdgcn_sched_barrier(0);
+      read(rd, q + 1, (q + 1) & 1);
+      __builtin_amdgcn_sched_barrier(0);
+      products(q & 1, wr, q == 0 ? PQ : -1);
+    }
+    lin_dma_sync();
+  };
+  if (steps > 0) {
+    begin();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) piece(lds, i);
+    lin_dma_sync();
+    step(lds, lds + STAGE, LinFlag<true>{});
+    for (int s = 1; s < steps; ++s) step(lds + (s & 1) * STAGE, lds + (~s & 1) * STAGE, LinFlag<false>{});
+    products(1, lds, -1);
   }
-  lin_dma_sync();
   lin_write_out<T, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                   j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
 }
