@@ -197,6 +197,13 @@ template <bool FAST> __device__ __forceinline__ void lin_act8(float (&v)[8], int
 #undef TNV3_LIN_ACT_CASE
 }
 
+// A raw buffer descriptor's range for `left` bytes up to the operand's end (negative: none): at most 2^31 - 1, in 32-bit scalar operations
+__device__ __forceinline__ unsigned lin_range(long left) {
+  const int hi = (int)(left >> 32);
+  const unsigned lo = (unsigned)left;
+  return hi < 0 ? 0u : (hi > 0 || lo > 0x7fffffffu ? 0x7fffffffu : lo);
+}
+
 // ---- LDS tiles
 // Position (in 16-bit elements) of 8-element chunk c of row r in an LDS tile.  LDS has 64 banks of 4 bytes: a 16-byte fragment read serves 16 lanes
 // (16 rows of one chunk) per clock if they name 16 different 16-byte slots of 256 bytes, the transposing read 32 lanes (4 rows of k, two 32-byte

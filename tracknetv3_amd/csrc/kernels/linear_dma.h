@@ -53,8 +53,7 @@ struct LinDma {
   }
   // the step's descriptor; then the next step's base
   __device__ __forceinline__ tnv3_rsrc_t begin() {
-    const unsigned bytes = left <= 0 ? 0u : (left > 0x7fffffffl ? 0x7fffffffu : (unsigned)left);
-    const tnv3_rsrc_t r = tnv3_make_rsrc(base, bytes);
+    const tnv3_rsrc_t r = tnv3_make_rsrc(base, lin_range(left));
     base += step;
     left -= step;
     return r;
@@ -98,13 +97,13 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     db.init(p.b, KSB ? kbeg * p.ldb + j0 : j0 * p.ldb + kbeg, KSB ? p.kk * p.ldb : p.rows_j * p.ldb, p.ldb, wave, lane);
   }
   // the stage being filled: its descriptors, what is left of the contraction there
-  long kleft = kend - kbeg;
+  int kleft = (int)(kend - kbeg);
   tnv3_rsrc_t ra, rb;
   int kl = 0;
   auto begin = [&]() {
     ra = da.begin();
     rb = db.begin();
-    kl = kleft > BK ? BK : (kleft > 0 ? (int)kleft : 0);
+    kl = kleft > 0 ? kleft : 0;
     kleft -= BK;
   };
   constexpr int NA = LinDma<KSA, BI, Cfg::NW>::N, NP = NA + LinDma<KSB, BJ, Cfg::NW>::N;
@@ -152,7 +151,6 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
   // transposing read wait for all loads in flight.  The fences keep the reads ahead of the products: left alone, the scheduler puts each read right
   // in front of its use.)
   auto step = [&](const unsigned short* __restrict__ rd, unsigned short* __restrict__ wr, auto first) {
-    begin();                                    // (beyond the last step: zeros into a stage that is not read)
     read(rd, 0, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (decltype(first)::value) {
@@ -167,6 +165,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       read(rd, q + 1, (q + 1) & 1);
       __builtin_amdgcn_sched_barrier(0);
       products(q & 1, wr, q == 0 ? PQ : -1);
+      if (q == 1) begin();                      // the next step's descriptors (beyond the last step: zeros into a stage that is not read)
     }
     lin_dma_sync();
   };
@@ -174,9 +173,16 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     begin();
 #pragma unroll
     for (int i = 0; i < NP; ++i) piece(lds, i);
+    begin();
     lin_dma_sync();
+    // (two steps per turn: the stages' addresses are constants then, nothing is computed between the barrier and the first reads)
     step(lds, lds + STAGE, LinFlag<true>{});
-    for (int s = 1; s < steps; ++s) step(lds + (s & 1) * STAGE, lds + (~s & 1) * STAGE, LinFlag<false>{});
+    int s = 1;
+    for (; s + 1 < steps; s += 2) {
+      step(lds + STAGE, lds, LinFlag<false>{});
+      step(lds, lds + STAGE, LinFlag<false>{});
+    }
+    if (s < steps) step(lds + STAGE, lds, LinFlag<false>{});
     products(1, lds, -1);
   }
   lin_write_out<T, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,

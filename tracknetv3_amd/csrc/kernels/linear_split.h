@@ -80,7 +80,7 @@ struct LinSplitLoader {
     }
   }
   __device__ __forceinline__ tnv3_rsrc_t rsrc() const {
-    return tnv3_make_rsrc(base, left <= 0 ? 0u : (left > 0x7fffffffl ? 0x7fffffffu : (unsigned)left));
+    return tnv3_make_rsrc(base, lin_range(left));
   }
   __device__ __forceinline__ void load(tnv3_rsrc_t r, int i) {
     const f32x4 a = lin_buf_load4(r, off[i], 0), b = lin_buf_load4(r, off[i], 16);
