@@ -37,6 +37,12 @@ __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinBf16
 __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinF16) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(lin_h8, a), __builtin_bit_cast(lin_h8, b), c, 0, 0, 0);
 }
+__device__ __forceinline__ f32x4 lin_mfma16(lin_s8 a, lin_s8 b, f32x4 c, LinBf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf8, a), __builtin_bit_cast(lin_bf8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 lin_mfma16(lin_s8 a, lin_s8 b, f32x4 c, LinF16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lin_h8, a), __builtin_bit_cast(lin_h8, b), c, 0, 0, 0);
+}
 // Transposing LDS read: within each group of 16 lanes, lane q's address names 4 elements of row q >> 2 (columns 4 (q & 3) ..), and lane q
 // receives column q of the four rows.
 __device__ __forceinline__ lin_s4 lin_lds_tr4(const unsigned short* p) {
@@ -61,6 +67,8 @@ __device__ __forceinline__ f32x4 lin_buf_load4(tnv3_rsrc_t r, unsigned voffset, 
 #else
 __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinBf16) { return emu_mfma_32x32x16(a, b, c, emu_bf16_up); }
 __device__ __forceinline__ f32x16 lin_mfma(lin_s8 a, lin_s8 b, f32x16 c, LinF16) { return emu_mfma_32x32x16(a, b, c, emu_f16_up); }
+__device__ __forceinline__ f32x4 lin_mfma16(lin_s8 a, lin_s8 b, f32x4 c, LinBf16) { return emu_mfma_16x16x32(a, b, c, emu_bf16_up); }
+__device__ __forceinline__ f32x4 lin_mfma16(lin_s8 a, lin_s8 b, f32x4 c, LinF16) { return emu_mfma_16x16x32(a, b, c, emu_f16_up); }
 __device__ __forceinline__ lin_s4 lin_lds_tr4(const unsigned short* p) { return emu_lds_tr4(p); }
 __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinBf16) { return (unsigned)emu_bf16_dn(a) | (unsigned)emu_bf16_dn(b) << 16; }
 __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) { return (unsigned)emu_f16_dn(a) | (unsigned)emu_f16_dn(b) << 16; }
@@ -211,6 +219,8 @@ __device__ __forceinline__ unsigned lin_range(long left) {
 // bits half of all LDS cycles were conflicts.)
 template <int BK> __device__ __forceinline__ int lin_pos_kc(int r, int c) { return r * BK + ((c ^ (BK == 64 ? (r >> 1) & 7 : (r >> 2) & 3)) << 3); }
 __device__ __forceinline__ int lin_pos_ks(int k, int c, int ld) { return k * ld + ((c ^ (ld == 64 ? (k & 2) << 1 : (k & 3) << 2)) << 3); }
+// the same for fragments of 16 rows and 32 of k, whose transposing read takes rows k and k + 8 of one 32-byte piece at a time (rows of 128 elements and more)
+__device__ __forceinline__ int lin_pos_ks16(int k, int c, int ld) { return k * ld + ((c ^ (((k & 3) << 2) | ((k & 8) >> 2))) << 3); }
 
 // fragments of one operand: rows base + 32 t + (l & 31), k = 16 s + 8 (l >> 5) + 0..7
 template <bool KS, int BK, int ROWS>
@@ -222,6 +232,29 @@ __device__ __forceinline__ lin_s8 lin_frag(const unsigned short* tile, int base,
   const lin_s4 lo = lin_lds_tr4(p), hi = lin_lds_tr4(p + 4 * ROWS);
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
+
+// Fragments of one operand, 16x16x32: rows base + 16 t + (l & 15), k = 32 s + 8 (l >> 4) + 0..7, from a stage of 64 of k (base a multiple of 64).
+// The lane's part of the address is computed once: k-contiguous rows differ by constants only, k-strided ones by one exclusive-or per 16 rows.
+template <bool KS, int ROWS>
+struct LinFrag16 {
+  int off[KS ? 1 : 2];      // bytes
+  __device__ __forceinline__ void init(int base, int lane) {
+    const int q = lane & 15, g = lane >> 4;
+    if (KS) {
+      off[0] = 2 * (lin_pos_ks16(8 * g + (q >> 2), (base >> 3) + ((q & 3) >> 1), ROWS) + (q & 1) * 4);
+    } else {
+#pragma unroll
+      for (int s = 0; s < (KS ? 1 : 2); ++s) off[s] = 2 * (base * 64 + lin_pos_kc<64>(q, 4 * s + g));
+    }
+  }
+  __device__ __forceinline__ lin_s8 get(const unsigned short* tile, int t, int s) const {
+    const char* p = reinterpret_cast<const char*>(tile);
+    if (!KS) return *reinterpret_cast<const lin_s8*>(p + off[KS ? 0 : s] + t * 16 * 64 * 2);
+    const unsigned short* r = reinterpret_cast<const unsigned short*>(p + (off[0] ^ (t << 5)) + s * 32 * ROWS * 2);
+    const lin_s4 lo = lin_lds_tr4(r), hi = lin_lds_tr4(r + 4 * ROWS);      // row k + 4 has row k's order
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+};
 
 // ---- one product's arguments
 struct LinGemmArgs {
@@ -310,10 +343,10 @@ __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&
 // layout gives a lane one column: read back by rows a lane holds eight consecutive columns, so bias, residual and outputs move in 16-byte pieces.
 // GATED: a wave's first TN/2 column tiles are the gate's, the last TN/2 the other factor's of the same outputs.
 constexpr int kLinSlabLd = 68, kLinSlabFloats = 32 * kLinSlabLd;
-template <class T, int TM, int TN, bool GATED>
-__device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16 (&acc)[TM][TN], float* slab, int lane, long i0, long j0, int sp) {
+// put(slab, tm, left, right): the accumulators of rows 32 tm .. and column tiles (of 32) left, right into the slab.
+template <class T, int TM, int TN, bool GATED, class Put>
+__device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, float* slab, int lane, long i0, long j0, int sp) {
   static_assert(TN % 2 == 0, "a slab is two column tiles wide");
-  const int half = lane >> 5, col = lane & 31;
   constexpr int LPR = GATED ? 4 : 8, RPP = 64 / LPR;        // lanes per row, rows per pass
   const int lr = lane / LPR, c8 = (lane % LPR) * 8;
 #pragma unroll
@@ -327,15 +360,8 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16
     }
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-      const f32x16& lo = acc[tm][GATED ? c : 2 * c];
-      const f32x16& hi = acc[tm][GATED ? c + TN / 2 : 2 * c + 1];
       lin_wave_sync();
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        float* d = slab + ((r & 3) + 8 * (r >> 2) + 4 * half) * kLinSlabLd + col;
-        d[0] = lo[r];
-        d[32] = hi[r];
-      }
+      put(slab, tm, GATED ? c : 2 * c, GATED ? c + TN / 2 : 2 * c + 1);
       lin_wave_sync();
 #pragma unroll 1
       for (int pass = 0; pass < 32 / RPP; ++pass) {
@@ -362,6 +388,26 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, const f32x16
       }
     }
   }
+}
+
+template <int TM, int TN>
+__device__ __forceinline__ void lin_put32(const f32x16 (&acc)[TM][TN], float* slab, int tm, int left, int right, int lane) {
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    float* d = slab + ((r & 3) + 8 * (r >> 2) + 4 * (lane >> 5)) * kLinSlabLd + (lane & 31);
+    d[0] = acc[tm][left][r];
+    d[32] = acc[tm][right][r];
+  }
+}
+template <int XM, int YN>
+__device__ __forceinline__ void lin_put16(const f32x4 (&acc)[XM][YN], float* slab, int tm, int left, int right, int lane) {
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        slab[(16 * x + 4 * (lane >> 4) + r) * kLinSlabLd + 16 * y + (lane & 15)] = acc[2 * tm + x][2 * (y < 2 ? left : right) + (y & 1)][r];
 }
 
 // ---- joins the partial sums of a split contraction in a fixed order and finishes them: one work-item per 8 columns of a row

@@ -40,8 +40,8 @@ struct LinDma {
       const int piece = wave * N + i;
       if (KS) {
         constexpr int LPR = ROWS / 8;
-        static_assert(ROWS >= 128, "lin_pos_ks's order for these rows");
-        const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ ((k & 3) << 2);
+        static_assert(ROWS >= 128, "lin_pos_ks16's order");
+        const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ (((k & 3) << 2) | ((k & 8) >> 2));
         off[i] = (unsigned)(k * (int)(2 * ld) + c * 16);
       } else {
         static_assert(N % 2 == 0, "piece i of a wave is odd where i is");
@@ -113,32 +113,43 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     else db.piece(rb, into + BI * BK, i - NA, kl, wave);
   };
 
-  f32x16 acc[TM][TN];
+  // Quarter q of a step: 32 of the contraction (q / 2) for half of the wave's columns (q % 2).  16x16x32 products: the larger form writes and reads
+  // twice the accumulator bytes per product, and at full tilt the card's power, not the issue of products, is the limit.
+  constexpr int XM = 2 * TM, YN = 2 * TN;             // 16-row / 16-column tiles of the wave
+  f32x4 acc[XM][YN];
 #pragma unroll
-  for (int x = 0; x < TM; ++x)
+  for (int x = 0; x < XM; ++x)
 #pragma unroll
-    for (int y = 0; y < TN; ++y)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.0f;
+    for (int y = 0; y < YN; ++y) acc[x][y] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 
-  lin_s8 fa[2][TM], fb[2][TN];
-  auto read = [&](const unsigned short* t, int q, int set) {
+  lin_s8 fa[2][XM], fb[2][TN];
+  LinFrag16<KSA, BI> ga;
+  LinFrag16<KSB, BJ> gb;
+  ga.init(wi * TM * 32, lane);
+  gb.init(wj * TN * 32, lane);
+  auto read = [&](const unsigned short* t, int q) {
+    // (opaque: an exclusive-or per fragment stays where it is instead of occupying a register per address across the loop)
+    if (KSA) TNV3_OPAQUE_V(ga.off[0]);
+    if (KSB) TNV3_OPAQUE_V(gb.off[0]);
+    if (q % 2 == 0) {
 #pragma unroll
-    for (int x = 0; x < TM; ++x) fa[set][x] = lin_frag<KSA, BK, BI>(t, wi * TM * 32, x, q, lane);
+      for (int x = 0; x < XM; ++x) fa[q / 2][x] = ga.get(t, x, q / 2);
+    }
 #pragma unroll
-    for (int y = 0; y < TN; ++y) fb[set][y] = lin_frag<KSB, BK, BJ>(t + BI * BK, wj * TN * 32, y, q, lane);
+    for (int y = 0; y < TN; ++y) fb[q % 2][y] = gb.get(t + BI * BK, (q % 2) * TN + y, q / 2);
   };
   // the products of one quarter, PQ pieces of direct loads (first .. first + PQ - 1) between them: a wave's loads queue behind those of the CU's other
   // waves (16 clocks of the address path each), so they are spread over two quarters instead of standing in front of the products
-  constexpr int PQ = 4, GAP = TM * TN / PQ;
+  constexpr int PQ = 4, GAP = XM * TN / PQ;
   static_assert(Q == 4 && NP <= 2 * PQ && GAP > 0, "a stage's pieces: two quarters");
-  auto products = [&](int set, unsigned short* into, int first) {
+  auto products = [&](int q, unsigned short* into, int first) {
 #pragma unroll
     for (int y = 0; y < TN; ++y)
 #pragma unroll
-      for (int x = 0; x < TM; ++x) {
-        const int m = y * TM + x;
-        acc[x][y] = lin_mfma(fa[set][x], fb[set][y], acc[x][y], T{});
+      for (int x = 0; x < XM; ++x) {
+        const int m = y * XM + x;
+        f32x4& c = acc[x][(q % 2) * TN + y];
+        c = lin_mfma16(fa[q / 2][x], fb[q % 2][y], c, T{});
         if (first >= 0 && m % GAP == GAP - 1 && m / GAP < PQ) {
           __builtin_amdgcn_sched_barrier(0);
           piece(into, first + m / GAP);
@@ -151,20 +162,20 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
   // transposing read wait for all loads in flight.  The fences keep the reads ahead of the products: left alone, the scheduler puts each read right
   // in front of its use.)
   auto step = [&](const unsigned short* __restrict__ rd, unsigned short* __restrict__ wr, auto first) {
-    read(rd, 0, 0);
+    read(rd, 0);
     __builtin_amdgcn_sched_barrier(0);
     if (decltype(first)::value) {
 #pragma unroll
       for (int i = 0; i < PQ; ++i) piece(wr, i);
     } else {
-      products(1, wr, 0);
+      products(3, wr, 0);
     }
 #pragma unroll
     for (int q = 0; q + 1 < Q; ++q) {
       __builtin_amdgcn_sched_barrier(0);
-      read(rd, q + 1, (q + 1) & 1);
+      read(rd, q + 1);
       __builtin_amdgcn_sched_barrier(0);
-      products(q & 1, wr, q == 0 ? PQ : -1);
+      products(q, wr, q == 0 ? PQ : -1);
       if (q == 1) begin();                      // the next step's descriptors (beyond the last step: zeros into a stage that is not read)
     }
     lin_dma_sync();
@@ -183,9 +194,10 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       step(lds, lds + STAGE, LinFlag<false>{});
     }
     if (s < steps) step(lds + STAGE, lds, LinFlag<false>{});
-    products(1, lds, -1);
+    products(3, lds, -1);
   }
-  lin_write_out<T, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
+  auto put = [&](float* slab, int tm, int left, int right) { lin_put16(acc, slab, tm, left, right, lane); };
+  lin_write_out<T, TM, TN, GATED>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                   j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
 }
 

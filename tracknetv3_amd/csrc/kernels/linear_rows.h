@@ -12,23 +12,10 @@
 
 namespace tnv3 {
 
-#ifndef TNV3_EMU
 typedef unsigned lin_u4_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, LinBf16) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(lin_bf8, a), __builtin_bit_cast(lin_bf8, b), c, 0, 0, 0);
+template <class T> __device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, T) {
+  return lin_mfma16(__builtin_bit_cast(lin_s8, a), __builtin_bit_cast(lin_s8, b), c, T{});
 }
-__device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, LinF16) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(lin_h8, a), __builtin_bit_cast(lin_h8, b), c, 0, 0, 0);
-}
-#else
-typedef unsigned lin_u4_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, LinBf16) {
-  return emu_mfma_16x16x32(__builtin_bit_cast(lin_s8, a), __builtin_bit_cast(lin_s8, b), c, emu_bf16_up);
-}
-__device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, LinF16) {
-  return emu_mfma_16x16x32(__builtin_bit_cast(lin_s8, a), __builtin_bit_cast(lin_s8, b), c, emu_f16_up);
-}
-#endif
 // fp32: lane l's four k values are 4 (l >> 4) + 0..3 of 16; product e takes k = e, 4 + e, 8 + e, 12 + e of both operands
 __device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, float) {
 #pragma unroll

@@ -248,7 +248,8 @@ __device__ __forceinline__ void lin_split_product(const LinGemmArgs& p, int bloc
     __syncthreads();
     if (redo) pass(LinFlag<true>{});
   }
-  lin_write_out<float, TM, TN, GATED>(p, acc, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
+  auto put = [&](float* slab, int tm, int left, int right) { lin_put32(acc, slab, tm, left, right, lane); };
+  lin_write_out<float, TM, TN, GATED>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                       j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
 }
 
