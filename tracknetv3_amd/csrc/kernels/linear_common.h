@@ -422,6 +422,7 @@ __device__ __forceinline__ void lin_join(const LinGemmArgs& p, long block) {
   float v[8], u[8], q[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.0f;
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
     const float* part = p.part + ((long)s * p.rows_i + i) * p.rows_j + j;
     lin_load8<float>(part, q, vec, n);

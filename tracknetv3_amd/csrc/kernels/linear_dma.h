@@ -40,7 +40,7 @@ struct LinDma {
       const int piece = wave * N + i;
       if (KS) {
         constexpr int LPR = ROWS / 8;
-        static_assert(ROWS >= 128, "lin_pos_ks16's order");
+        static_assert(!KS || ROWS >= 128, "lin_pos_ks16's order");
         const int k = piece * (64 / LPR) + lane / LPR, c = (lane % LPR) ^ (((k & 3) << 2) | ((k & 8) >> 2));
         off[i] = (unsigned)(k * (int)(2 * ld) + c * 16);
       } else {

@@ -11,6 +11,7 @@ namespace tnv3 {
 
 using LinD256 = LinDmaCfg<2, 4, 4, 2>;          // 256 x 256, eight waves of 64 x 128: one workgroup per CU
 using LinD128 = LinDmaCfg<2, 2, 2, 2>;          // 128 x 128, four waves of 64 x 64: two workgroups per CU
+using LinD64 = LinDmaCfg<1, 2, 2, 1>;           // 64 x 64, two waves of 32 x 64: forward products of few tiles
 using LinF256 = LinSplitCfg<2, 2, 4, 2>;        // fp32: 256 x 128, eight waves of 64 x 64, one workgroup per CU (144 KB of LDS)
 using LinF128 = LinSplitCfg<1, 2, 4, 1>;        // fp32: 128 x 64, four waves of 32 x 64, two workgroups per CU
 
@@ -21,44 +22,92 @@ inline size_t lin_pad(size_t b) { return (b + 255) & ~(size_t)255; }
 inline int lin_size(int dtype) { return dtype == kLinF32 ? 4 : 2; }
 
 // One product's tiling.  Sizes and type decide, never the pointers, so that the workspace queries and the launches agree.
+enum { kTileSmall = 0, kTileNormal = 1, kTileWide = 2 };
 struct LinPlan {
-  bool wide;              // the 256-row tiles
-  int bi, bj, splits;
+  int tile, bi, bj, splits;
   long k_per_split, tiles;
   size_t part_bytes;
 };
 inline long lin_tiles(long rows_i, long rows_j, bool gated, int bi, int bj) {
   return ((rows_i + bi - 1) / bi) * (gated ? (rows_j / 2 + bj / 2 - 1) / (bj / 2) : (rows_j + bj - 1) / bj);
 }
-inline void lin_tile_shape(LinPlan& pl, int dtype, bool wide) {
-  pl.wide = wide;
-  pl.bi = wide ? 256 : 128;
-  pl.bj = dtype == kLinF32 ? (wide ? 128 : 64) : (wide ? 256 : 128);
+// What a launch takes, in microseconds, from timings of 16 to 4096 tiles at contractions of 256 to 2048 on 256 CUs: a workgroup's 64 of the contraction
+// take `lat` alone on its CU and `thr` of the CU's time among others, `occ` of them share a CU, a launch costs `fix`, a further round of
+// workgroups `again`.  16-bit, per 64: 64 x 64 tiles 0.25-0.28 alone, 1.30 with 8 a CU; 128 x 128 0.40-0.8 alone, 3.1 with 8 a CU; 256 x 256 1.1-1.8,
+// 6.1 with 4 a CU.  fp32: 128 x 64 1.7-2.2, 12.6 with 8 a CU; 256 x 128 3.4-4.4, 18.8 with 4 a CU.  Adding the parts of a split contraction: a
+// launch of 2 and its bytes at 4.5 TB/s.
+struct LinCost { int bi, bj, occ; double thr, lat, fix, again; };
+inline const LinCost& lin_cost(int dtype, int tile) {
+  static const LinCost t[2][3] = {{{64, 64, 5, 0.165, 0.27, 4.0, 1.0}, {128, 128, 2, 0.45, 0.55, 5.0, 2.0}, {256, 256, 1, 1.55, 1.55, 8.0, 4.0}},
+                                  {{0, 0, 0, 0, 0, 0, 0}, {128, 64, 2, 1.6, 1.9, 4.0, 1.5}, {256, 128, 1, 4.5, 4.5, 9.0, 4.0}}};
+  return t[dtype == kLinF32 ? 1 : 0][tile];
 }
-inline long lin_wide_tiles(int dtype, long rows_i, long rows_j, bool gated) { return lin_tiles(rows_i, rows_j, gated, 256, dtype == kLinF32 ? 128 : 256); }
-// others: tiles of a product in the same launch
-inline void lin_split_plan(LinPlan& pl, long rows_i, long rows_j, long kk, bool gated, long others) {
-  pl.tiles = lin_tiles(rows_i, rows_j, gated, pl.bi, pl.bj);
-  // fewer tiles than CUs: the contraction is split so that all take part, as long as a part keeps 4 steps of 64
-  const long tiles = pl.tiles + others, cus = num_cus(), step = 64, steps = (kk + step - 1) / step;
-  long s = 1;
-  if (tiles < cus) {
-    s = cus / tiles;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 32) s = 32;
-    if (s < 1) s = 1;
-  }
-  const long per = (steps + s - 1) / s;
+inline double lin_steps_time(const LinCost& c, long groups, long steps) {
+  const long per = (groups + num_cus() - 1) / num_cus(), full = per / c.occ, rem = per % c.occ;
+  const double whole = c.occ * c.thr > c.lat ? c.occ * c.thr : c.lat, part = rem * c.thr > c.lat ? rem * c.thr : c.lat;
+  return c.fix + steps * (full * whole + (rem ? part : 0.0)) + c.again * (full + (rem ? 1 : 0) - 1);
+}
+constexpr int kLinSplits[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32};
+inline double lin_join_bytes(long rows_i, long rows_j, long s) { return s > 1 ? 8.0 * s * rows_i * rows_j : 0.0; }
+inline double lin_join_time(double bytes) { return bytes > 0 ? 2.0 + bytes / 4.5e6 : 0.0; }
+inline void lin_set_plan(LinPlan& pl, int dtype, int tile, long rows_i, long rows_j, long kk, bool gated, long s) {
+  const LinCost& c = lin_cost(dtype, tile);
+  pl.tile = tile;
+  pl.bi = c.bi;
+  pl.bj = c.bj;
+  pl.tiles = lin_tiles(rows_i, rows_j, gated, c.bi, c.bj);
+  const long steps = (kk + 63) / 64, per = (steps + s - 1) / s;
   pl.splits = (int)((steps + per - 1) / per);
-  pl.k_per_split = per * step;
+  pl.k_per_split = per * 64;
   pl.part_bytes = pl.splits > 1 ? lin_pad((size_t)pl.splits * rows_i * rows_j * 4) : 0;
 }
+// the forward product: the tile and the number of parts of the contraction with the least expected time
 inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated) {
   LinPlan pl;
-  // at least a 256-row tile for every CU: half the LDS and L2 traffic per product
-  lin_tile_shape(pl, dtype, lin_wide_tiles(dtype, rows_i, rows_j, gated) >= num_cus());
-  lin_split_plan(pl, rows_i, rows_j, kk, gated, 0);
+  double best = 0;
+  int tile = kTileNormal;
+  long split = 0;
+  const long steps = (kk + 63) / 64;
+  for (int t = dtype == kLinF32 ? kTileNormal : kTileSmall; t <= kTileWide; ++t) {
+    const LinCost& c = lin_cost(dtype, t);
+    const long tiles = lin_tiles(rows_i, rows_j, gated, c.bi, c.bj);
+    for (long s : kLinSplits) {
+      if (s > 1 && (s > steps || tiles * s > 4 * num_cus())) break;
+      const double e = lin_steps_time(c, tiles * s, (steps + s - 1) / s) + lin_join_time(lin_join_bytes(rows_i, rows_j, s));
+      if (split == 0 || e < best) { best = e; tile = t; split = s; }
+    }
+  }
+  lin_set_plan(pl, dtype, tile, rows_i, rows_j, kk, gated, split);
   return pl;
+}
+// The two products of a backward pass in one launch: the longest workgroup and the work per CU bound the time; the product with the longest
+// workgroups is split further as long as that helps.
+inline void lin_pair_plan(LinPlan& dx, LinPlan& dw, int dtype, long rows, int k, int n2) {
+  const long ri[2] = {rows, n2}, steps[2] = {((long)n2 + 63) / 64, (rows + 63) / 64};
+  double best = -1;
+  int tile = kTileNormal;
+  int choice[2] = {0, 0};
+  for (int t = kTileNormal; t <= kTileWide; ++t) {
+    const LinCost& c = lin_cost(dtype, t);
+    const long tiles[2] = {lin_tiles(ri[0], k, false, c.bi, c.bj), lin_tiles(ri[1], k, false, c.bi, c.bj)};
+    int at[2] = {0, 0};
+    for (;;) {
+      const long s[2] = {kLinSplits[at[0]], kLinSplits[at[1]]}, n[2] = {(steps[0] + s[0] - 1) / s[0], (steps[1] + s[1] - 1) / s[1]};
+      const long groups = tiles[0] * s[0] + tiles[1] * s[1], per = (groups + num_cus() - 1) / num_cus();
+      const double share = (per < c.occ ? per : c.occ) * c.thr, each = share > c.lat ? share : c.lat;
+      const int longer = n[0] >= n[1] ? 0 : 1;
+      const double longest = n[longer] * each;
+      const double work = (tiles[0] * s[0] * (n[0] * c.thr + c.again / c.occ) + tiles[1] * s[1] * (n[1] * c.thr + c.again / c.occ)) / num_cus();
+      // one round of workgroups: the longest; several: the work, and on average a part of the longest in which CUs run dry
+      double e = groups <= (long)num_cus() * c.occ || work + 0.4 * longest < longest ? longest : work + 0.4 * longest;
+      e += c.fix + lin_join_time(lin_join_bytes(ri[0], k, s[0]) + lin_join_bytes(ri[1], k, s[1]));
+      if (best < 0 || e < best) { best = e; tile = t; choice[0] = at[0]; choice[1] = at[1]; }
+      if (at[longer] + 1 >= (int)(sizeof(kLinSplits) / sizeof(int)) || kLinSplits[at[longer] + 1] > steps[longer] || groups > 8 * num_cus()) break;
+      ++at[longer];
+    }
+  }
+  lin_set_plan(dx, dtype, tile, rows, k, n2, false, kLinSplits[choice[0]]);
+  lin_set_plan(dw, dtype, tile, n2, k, rows, false, kLinSplits[choice[1]]);
 }
 inline void lin_apply(LinGemmArgs& p, const LinPlan& pl, float* part) {
   p.splits = pl.splits;
@@ -134,10 +183,11 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   if (int rc = pad.launch(L)) return rc;
   int rc;
   if constexpr (sizeof(T) == 2) {
-    if (l.plan.wide) rc = L.launch(lin_dma_kernel<LinD256, T, GATED>, (int)grid, LinD256::NT, p);
+    if (l.plan.tile == kTileWide) rc = L.launch(lin_dma_kernel<LinD256, T, GATED>, (int)grid, LinD256::NT, p);
+    else if (l.plan.tile == kTileSmall) rc = L.launch(lin_dma_kernel<LinD64, T, GATED>, (int)grid, LinD64::NT, p);
     else rc = L.launch(lin_dma_kernel<LinD128, T, GATED>, (int)grid, LinD128::NT, p);
   } else {
-    if (l.plan.wide) rc = L.launch(lin_split_kernel<LinF256, GATED>, (int)grid, LinF256::NT, p);
+    if (l.plan.tile == kTileWide) rc = L.launch(lin_split_kernel<LinF256, GATED>, (int)grid, LinF256::NT, p);
     else rc = L.launch(lin_split_kernel<LinF128, GATED>, (int)grid, LinF128::NT, p);
   }
   if (rc || p.splits == 1) return rc;
@@ -148,7 +198,7 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
 // row blocks of the element-wise pass: about four workgroups per CU, at least 8 rows (one per work-item) each, and no more blocks than the final column
 // sums can add quickly
 inline long lin_dz_rows(long rows, int n) {
-  const long jt = (n + 255) / 256, cap = rows / 128 < 64 ? 64 : (rows / 128 > 512 ? 512 : rows / 128);
+  const long jt = (n + 255) / 256, cap = rows / 128 < 256 ? 256 : (rows / 128 > 512 ? 512 : rows / 128);
   long blocks = 4l * num_cus() / jt;
   blocks = blocks < 1 ? 1 : (blocks > cap ? cap : blocks);
   const long per = ((rows + blocks - 1) / blocks + 7) / 8 * 8;
@@ -158,11 +208,7 @@ struct LinBackwardLayout { LinPlan dx, dw; size_t dz, sums, w, x, part_dx, part_
 inline LinBackwardLayout lin_backward_layout(long rows, int k, int n, int act, int dtype, bool gated) {
   const int n2 = gated ? 2 * n : n;
   LinBackwardLayout l;
-  const bool wide = lin_wide_tiles(dtype, rows, k, false) + lin_wide_tiles(dtype, n2, k, false) >= num_cus();
-  lin_tile_shape(l.dx, dtype, wide);
-  lin_tile_shape(l.dw, dtype, wide);
-  lin_split_plan(l.dx, rows, k, n2, false, lin_tiles(n2, k, false, l.dw.bi, l.dw.bj));
-  lin_split_plan(l.dw, n2, k, rows, false, lin_tiles(rows, k, false, l.dx.bi, l.dx.bj));
+  lin_pair_plan(l.dx, l.dw, dtype, rows, k, n2);
   const long per = lin_dz_rows(rows, n);
   l.dz = 0;
   l.sums = l.dz + (gated || act != kActNone ? lin_pad((size_t)rows * lin_ld(dtype, n2) * lin_size(dtype)) : lin_pad_bytes(dtype, rows, n2));
@@ -221,10 +267,10 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   if (int rc = lin_grid_check(grid > joins_dx + joins_dw ? grid : joins_dx + joins_dw)) return rc;
   int rc;
   if constexpr (sizeof(T) == 2) {
-    if (l.dx.wide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
+    if (l.dx.tile == kTileWide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
     else rc = L.launch(lin_dma_pair_kernel<LinD128, T>, (int)grid, LinD128::NT, q);
   } else {
-    if (l.dx.wide) rc = L.launch(lin_split_pair_kernel<LinF256>, (int)grid, LinF256::NT, q);
+    if (l.dx.tile == kTileWide) rc = L.launch(lin_split_pair_kernel<LinF256>, (int)grid, LinF256::NT, q);
     else rc = L.launch(lin_split_pair_kernel<LinF128>, (int)grid, LinF128::NT, q);
   }
   if (rc || joins_dx + joins_dw == 0) return rc;
