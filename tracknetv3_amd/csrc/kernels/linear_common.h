@@ -105,6 +105,12 @@ __device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinF16) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) { v[2 * i] = lin_f16_up((unsigned short)(q[i] & 0xffffu)); v[2 * i + 1] = lin_f16_up((unsigned short)(q[i] >> 16)); }
 }
+// from the registers of a 16-byte load (fp32: two)
+template <class T> __device__ __forceinline__ void lin_unpack8(const lin_u4 (&q)[1], float (&v)[8], T) { lin_unpack8(q[0], v, T{}); }
+__device__ __forceinline__ void lin_unpack8(const lin_u4 (&q)[2], float (&v)[8], float) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = lin_bits(q[0][i]); v[4 + i] = lin_bits(q[1][i]); }
+}
 template <class T> __device__ __forceinline__ void lin_load8(const T* p, float (&v)[8], bool vec, int n) {
   if (vec) { lin_unpack8(*reinterpret_cast<const lin_u4*>(p), v, T{}); return; }
 #pragma unroll
@@ -341,50 +347,139 @@ __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&
 
 // The write-out goes through LDS, 32 rows x 64 columns per wave at a time (a slab of its own: no workgroup barrier), because the accumulator
 // layout gives a lane one column: read back by rows a lane holds eight consecutive columns, so bias, residual and outputs move in 16-byte pieces.
+// A slab's residual is loaded before the exchange.  Widths that are no whole pieces go element by element.
 // GATED: a wave's first TN/2 column tiles are the gate's, the last TN/2 the other factor's of the same outputs.
 constexpr int kLinSlabLd = 68, kLinSlabFloats = 32 * kLinSlabLd;
-// put(slab, tm, left, right): the accumulators of rows 32 tm .. and column tiles (of 32) left, right into the slab.
-template <class T, int TM, int TN, bool GATED, class Put>
+// put(slab, tm, left, right): the accumulators of rows 32 tm .. and column tiles (of 32) left, right into the slab.  PLAIN: the sums alone (a backward pass: no bias, activation, residual, pre-activation).
+template <class T, int TM, int TN, bool GATED, bool PLAIN, class Put>
 __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, float* slab, int lane, long i0, long j0, int sp) {
   static_assert(TN % 2 == 0, "a slab is two column tiles wide");
-  constexpr int LPR = GATED ? 4 : 8, RPP = 64 / LPR;        // lanes per row, rows per pass
-  const int lr = lane / LPR, c8 = (lane % LPR) * 8;
+  constexpr int LPR = GATED ? 4 : 8, RPP = 64 / LPR, NP = 32 / RPP, NG = 2;        // lanes per row, rows per pass, passes, at a time
+  constexpr bool FAST = sizeof(T) == 2;
+  const long cols = GATED ? p.f : p.rows_j;
+  float* part = p.part + (long)sp * p.rows_i * p.rows_j;
 #pragma unroll
   for (int c = 0; c < TN / 2; ++c) {
     // linear: columns j0 + 64 c ..; gated: outputs j0 + 32 c .. (gate tile c, other factor's tile c + TN / 2)
-    const long j = j0 + (GATED ? 32 * c : 64 * c) + c8;
+    const long jc = j0 + (GATED ? 32 * c : 64 * c);
+    const int left = GATED ? c : 2 * c, right = GATED ? c + TN / 2 : 2 * c + 1;
+    const int lr = lane / LPR;
+    const long j = jc + (lane % LPR) * 8;
+    const bool in = j < cols;
     float b0[8], b1[8];
-    if (p.splits == 1) {
-      lin_bias8<T>(p, GATED && j >= p.f ? p.rows_j : j, b0);
-      if (GATED) lin_bias8<T>(p, j >= p.f ? p.rows_j : p.f + j, b1);
+    if (p.splits == 1) {                                     // (PLAIN: there is none, zeros)
+      lin_bias8<T>(p, in ? j : p.rows_j, b0);
+      if (GATED) lin_bias8<T>(p, in ? p.f + j : p.rows_j, b1);
     }
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
-      lin_wave_sync();
-      put(slab, tm, GATED ? c : 2 * c, GATED ? c + TN / 2 : 2 * c + 1);
-      lin_wave_sync();
+      const long ir = i0 + 32 * tm + lr;                     // pass q: row ir + q RPP
+      if (!p.vec) {
+        lin_wave_sync();
+        put(slab, tm, left, right);
+        lin_wave_sync();
 #pragma unroll 1
-      for (int pass = 0; pass < 32 / RPP; ++pass) {
-        const int row = pass * RPP + lr;
-        const float* s = slab + row * kLinSlabLd + c8;
-        float v[8], u[8];
-        lin_load8<float>(s, v, true, 8);
-        if (GATED) lin_load8<float>(s + 32, u, true, 8);
-        const long i = i0 + 32 * tm + row;
-        if (p.splits > 1) {
-          if (i < p.rows_i) {
-            float* part = p.part + ((long)sp * p.rows_i + i) * p.rows_j;
-            const long lim = GATED ? p.f : p.rows_j;
-            const int n = lim - j < 8 ? (int)(lim - j) : 8;
-            const bool vec = p.vec && n == 8;
-            lin_store8<float>(part + j, v, vec, n);
-            if (GATED) lin_store8<float>(part + p.f + j, u, vec, n);
+        for (int q = 0; q < NP; ++q) {
+          const float* s = slab + (q * RPP + lr) * kLinSlabLd + (lane % LPR) * 8;
+          const long i = ir + q * RPP;
+          float v[8], u[8];
+          lin_load8<float>(s, v, true, 8);
+          if (GATED) lin_load8<float>(s + 32, u, true, 8);
+          if (p.splits > 1) {
+            const int n = cols - j < 8 ? (int)(cols - j) : 8;
+            if (i < p.rows_i) {
+              lin_store8<float>(part + i * p.rows_j + j, v, false, n);
+              if (GATED) lin_store8<float>(part + i * p.rows_j + p.f + j, u, false, n);
+            }
+          } else if (GATED) {
+            lin_finish_gated8<T>(p, i, j, v, u, b0, b1);
+          } else {
+            lin_finish8<T>(p, i, j, v, b0);
           }
-        } else if (GATED) {
-          lin_finish_gated8<T>(p, i, j, v, u, b0, b1);
-        } else {
-          lin_finish8<T>(p, i, j, v, b0);
         }
+        continue;
+      }
+      lin_u4 r[GATED ? 1 : NP][sizeof(T) / 2];
+      if (!GATED && !PLAIN && p.res && p.splits == 1) {
+#pragma unroll
+        for (int q = 0; q < (GATED ? 1 : NP); ++q)
+          if (in && ir + q * RPP < p.rows_i) {
+#pragma unroll
+            for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+              r[q][h] = reinterpret_cast<const lin_u4*>(static_cast<const T*>(p.res) + (ir + q * RPP) * p.rows_j + j)[h];
+          }
+      }
+      lin_wave_sync();
+      put(slab, tm, left, right);
+      lin_wave_sync();
+#pragma unroll
+      for (int q0 = 0; q0 < NP; q0 += NG) {
+        float v[NG][8], u[GATED ? NG : 1][8];
+#pragma unroll
+        for (int q = 0; q < NG; ++q) {
+          const float* s = slab + ((q0 + q) * RPP + lr) * kLinSlabLd + (lane % LPR) * 8;
+          lin_load8<float>(s, v[q], true, 8);
+          if (GATED) lin_load8<float>(s + 32, u[GATED ? q : 0], true, 8);
+        }
+        if (p.splits > 1) {
+#pragma unroll
+          for (int q = 0; q < NG; ++q)
+            if (in && ir + (q0 + q) * RPP < p.rows_i) {
+              float* o = part + (ir + (q0 + q) * RPP) * p.rows_j + j;
+              lin_store8<float>(o, v[q], true, 8);
+              if (GATED) lin_store8<float>(o + p.f, u[GATED ? q : 0], true, 8);
+            }
+          continue;
+        }
+#pragma unroll
+        for (int q = 0; q < (PLAIN ? 0 : NG); ++q)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[q][e] += b0[e];
+            if (GATED) u[GATED ? q : 0][e] += b1[e];
+          }
+        if (!PLAIN && p.pre) {
+#pragma unroll
+          for (int q = 0; q < NG; ++q)
+            if (in && ir + (q0 + q) * RPP < p.rows_i) {
+              const long o = (ir + (q0 + q) * RPP) * p.rows_j + j;
+              if (GATED) {
+                lin_store8<float>(static_cast<float*>(p.pre) + o, v[q], true, 8);
+                lin_store8<float>(static_cast<float*>(p.pre) + o + p.f, u[GATED ? q : 0], true, 8);
+              } else {
+                lin_store8<T>(static_cast<T*>(p.pre) + o, v[q], true, 8);
+              }
+            }
+        }
+        // the switch is wave-uniform and outside the elements' loops
+#define TNV3_LIN_ACT_CASE(A)                                                                        \
+    case A:                                                                                           \
+      _Pragma("unroll") for (int q = 0; q < NG; ++q)                                                  \
+        _Pragma("unroll") for (int e = 0; e < 8; ++e) v[q][e] = lin_act1<FAST>(v[q][e], A);           \
+      break;
+        switch (PLAIN ? kActNone : p.act) {
+          TNV3_LIN_ACT_CASE(kActLeaky) TNV3_LIN_ACT_CASE(kActSigmoid) TNV3_LIN_ACT_CASE(kActRelu) TNV3_LIN_ACT_CASE(kActSilu)
+          TNV3_LIN_ACT_CASE(kActGelu) TNV3_LIN_ACT_CASE(kActGeluTanh)
+          default: break;
+        }
+#undef TNV3_LIN_ACT_CASE
+#pragma unroll
+        for (int q = 0; q < NG; ++q)
+          if (in && ir + (q0 + q) * RPP < p.rows_i) {
+            if (GATED) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[q][e] *= u[GATED ? q : 0][e];
+              lin_store8<T>(static_cast<T*>(p.out) + (ir + (q0 + q) * RPP) * p.f + j, v[q], true, 8);
+            } else {
+              if (!PLAIN && p.res) {
+                float a[8];
+                lin_unpack8(r[GATED ? 0 : q0 + q], a, T{});
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[q][e] += a[e];
+              }
+              lin_store8<T>(static_cast<T*>(p.out) + (ir + (q0 + q) * RPP) * p.rows_j + j, v[q], true, 8);
+            }
+          }
       }
     }
   }

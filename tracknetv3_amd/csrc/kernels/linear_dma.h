@@ -197,7 +197,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
     products(3, lds, -1);
   }
   auto put = [&](float* slab, int tm, int left, int right) { lin_put16(acc, slab, tm, left, right, lane); };
-  lin_write_out<T, TM, TN, GATED>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
+  lin_write_out<T, TM, TN, GATED, KSB>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                   j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
 }
 

@@ -249,7 +249,7 @@ __device__ __forceinline__ void lin_split_product(const LinGemmArgs& p, int bloc
     if (redo) pass(LinFlag<true>{});
   }
   auto put = [&](float* slab, int tm, int left, int right) { lin_put32(acc, slab, tm, left, right, lane); };
-  lin_write_out<float, TM, TN, GATED>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
+  lin_write_out<float, TM, TN, GATED, KSB>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,
                                       j0 + (long)wj * TN * (GATED ? 16 : 32), sp);
 }
 
