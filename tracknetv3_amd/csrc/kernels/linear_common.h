@@ -60,6 +60,8 @@ __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) {
 }
 __device__ __forceinline__ float lin_f16_up(unsigned short h) { return (float)__builtin_bit_cast(_Float16, h); }
 __device__ __forceinline__ void lin_wave_sync() { __builtin_amdgcn_wave_barrier(); }
+// A store of 16 bytes reads its registers over several clocks: they stay unwritten for two wait states (see tnv3_buf_store_f4).
+__device__ __forceinline__ void lin_store_hold(lin_u4 q) { asm volatile("s_nop 1" : : "v"(q)); }
 // four fp32 at base + voffset + soffset, each checked against the descriptor's range (beyond it: 0)
 __device__ __forceinline__ f32x4 lin_buf_load4(tnv3_rsrc_t r, unsigned voffset, unsigned soffset) {
   return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(voffset + soffset), 0, 0));
@@ -74,6 +76,7 @@ __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinBf16) { retur
 __device__ __forceinline__ unsigned lin_pack2(float a, float b, LinF16) { return (unsigned)emu_f16_dn(a) | (unsigned)emu_f16_dn(b) << 16; }
 __device__ __forceinline__ float lin_f16_up(unsigned short h) { return emu_f16_up(h); }
 __device__ __forceinline__ void lin_wave_sync() { emu::wave_barrier(); }
+__device__ __forceinline__ void lin_store_hold(lin_u4) {}
 __device__ __forceinline__ f32x4 lin_buf_load4(tnv3_rsrc_t r, unsigned voffset, unsigned soffset) {
   f32x4 v;
   for (int e = 0; e < 4; ++e) {
@@ -132,6 +135,7 @@ template <class T> __device__ __forceinline__ void lin_store8(T* p, const float 
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = lin_pack2(v[2 * i], v[2 * i + 1], T{});
     *reinterpret_cast<lin_u4*>(p) = q;
+    lin_store_hold(q);
     return;
   }
 #pragma unroll
@@ -140,8 +144,11 @@ template <class T> __device__ __forceinline__ void lin_store8(T* p, const float 
 }
 template <> __device__ __forceinline__ void lin_store8<float>(float* p, const float (&v)[8], bool vec, int n) {
   if (vec) {
-    reinterpret_cast<f32x4*>(p)[0] = (f32x4){v[0], v[1], v[2], v[3]};
-    reinterpret_cast<f32x4*>(p)[1] = (f32x4){v[4], v[5], v[6], v[7]};
+    const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
+    reinterpret_cast<f32x4*>(p)[0] = a;
+    reinterpret_cast<f32x4*>(p)[1] = b;
+    lin_store_hold(__builtin_bit_cast(lin_u4, a));
+    lin_store_hold(__builtin_bit_cast(lin_u4, b));
     return;
   }
 #pragma unroll
