@@ -18,6 +18,9 @@ namespace tnv3 {
 typedef short lin_s8 __attribute__((ext_vector_type(8)));
 typedef short lin_s4 __attribute__((ext_vector_type(4)));
 typedef unsigned lin_u4 __attribute__((ext_vector_type(4)));
+// in memory: rows of odd widths start anywhere, and the hardware's 16-byte global accesses need no alignment beyond the element's
+typedef unsigned lin_u4_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float lin_f4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 template <bool V> struct LinFlag { static constexpr bool value = V; };
 template <int V> struct LinCount { static constexpr int value = V; };
@@ -99,7 +102,7 @@ __device__ __forceinline__ void lin_down(float f, float& o) { o = f; }
 // the fp32 value that an element of type T keeps of f
 template <class T> __device__ __forceinline__ float lin_round(float f) { T t; lin_down(f, t); return lin_up(t); }
 
-// ---- eight consecutive elements <-> fp32.  vec: p is 16-byte aligned and all eight exist; else the first `n` one by one (the rest 0).
+// ---- eight consecutive elements <-> fp32.  vec: all eight exist; else the first `n` one by one (the rest 0).
 __device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinBf16) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) { v[2 * i] = lin_bits(q[i] << 16); v[2 * i + 1] = lin_bits(q[i] & 0xffff0000u); }
@@ -115,13 +118,13 @@ __device__ __forceinline__ void lin_unpack8(const lin_u4 (&q)[2], float (&v)[8],
   for (int i = 0; i < 4; ++i) { v[i] = lin_bits(q[0][i]); v[4 + i] = lin_bits(q[1][i]); }
 }
 template <class T> __device__ __forceinline__ void lin_load8(const T* p, float (&v)[8], bool vec, int n) {
-  if (vec) { lin_unpack8(*reinterpret_cast<const lin_u4*>(p), v, T{}); return; }
+  if (vec) { lin_unpack8(*reinterpret_cast<const lin_u4_any*>(p), v, T{}); return; }
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = i < n ? lin_up(p[i]) : 0.0f;
 }
 template <> __device__ __forceinline__ void lin_load8<float>(const float* p, float (&v)[8], bool vec, int n) {
   if (vec) {
-    const f32x4 a = reinterpret_cast<const f32x4*>(p)[0], b = reinterpret_cast<const f32x4*>(p)[1];
+    const f32x4 a = reinterpret_cast<const lin_f4_any*>(p)[0], b = reinterpret_cast<const lin_f4_any*>(p)[1];
 #pragma unroll
     for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
     return;
@@ -134,7 +137,7 @@ template <class T> __device__ __forceinline__ void lin_store8(T* p, const float 
     lin_u4 q;
 #pragma unroll
     for (int i = 0; i < 4; ++i) q[i] = lin_pack2(v[2 * i], v[2 * i + 1], T{});
-    *reinterpret_cast<lin_u4*>(p) = q;
+    *reinterpret_cast<lin_u4_any*>(p) = q;
     lin_store_hold(q);
     return;
   }
@@ -145,8 +148,8 @@ template <class T> __device__ __forceinline__ void lin_store8(T* p, const float 
 template <> __device__ __forceinline__ void lin_store8<float>(float* p, const float (&v)[8], bool vec, int n) {
   if (vec) {
     const f32x4 a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
-    reinterpret_cast<f32x4*>(p)[0] = a;
-    reinterpret_cast<f32x4*>(p)[1] = b;
+    reinterpret_cast<lin_f4_any*>(p)[0] = a;
+    reinterpret_cast<lin_f4_any*>(p)[1] = b;
     lin_store_hold(__builtin_bit_cast(lin_u4, a));
     lin_store_hold(__builtin_bit_cast(lin_u4, b));
     return;
@@ -285,7 +288,6 @@ struct LinGemmArgs {
   int f;                  // gated: F
   int tiles_i, tiles_j, splits;
   long k_per_split;       // a multiple of the kernel's k step
-  bool vec;               // the outputs' rows (bias, residual) are whole 16-byte pieces
 };
 
 // block -> (tile_i, tile_j, split); false: beyond the last.  Workgroups go to the 8 XCDs in turn, and each XCD has its own L2: XCD x gets the x-th contiguous
@@ -310,7 +312,7 @@ template <class T>
 __device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j, float (&v)[8], const float (&bias)[8]) {
   if (i >= p.rows_i || j >= p.rows_j) return;
   const int n = p.rows_j - j < 8 ? (int)(p.rows_j - j) : 8;
-  const bool vec = p.vec && n == 8;
+  const bool vec = n == 8;
   const long o = i * p.rows_j + j;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
@@ -329,7 +331,7 @@ __device__ __forceinline__ void lin_finish_gated8(const LinGemmArgs& p, long i, 
                                                   const float (&bu)[8]) {
   if (i >= p.rows_i || j >= p.f) return;
   const int n = p.f - j < 8 ? (int)(p.f - j) : 8;
-  const bool vec = p.vec && n == 8;
+  const bool vec = n == 8;
 #pragma unroll
   for (int e = 0; e < 8; ++e) { g[e] += bg[e]; u[e] += bu[e]; }
   if (p.pre) {
@@ -346,7 +348,7 @@ template <class T>
 __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&b)[8]) {
   const long left = p.rows_j - j;
   const int n = left < 8 ? (left < 0 ? 0 : (int)left) : 8;
-  if (p.bias) lin_load8<T>(static_cast<const T*>(p.bias) + (n > 0 ? j : 0), b, p.vec && n == 8, n);
+  if (p.bias) lin_load8<T>(static_cast<const T*>(p.bias) + (n > 0 ? j : 0), b, n == 8, n);
   else
 #pragma unroll
     for (int e = 0; e < 8; ++e) b[e] = 0.0f;
@@ -354,9 +356,14 @@ __device__ __forceinline__ void lin_bias8(const LinGemmArgs& p, long j, float (&
 
 // The write-out goes through LDS, 32 rows x 64 columns per wave at a time (a slab of its own: no workgroup barrier), because the accumulator
 // layout gives a lane one column: read back by rows a lane holds eight consecutive columns, so bias, residual and outputs move in 16-byte pieces.
-// A slab's residual is loaded before the exchange.  Widths that are no whole pieces go element by element.
+// A slab's residual is loaded before the exchange.  Where a row ends inside a lane's eight columns, that lane goes element by element.
 // GATED: a wave's first TN/2 column tiles are the gate's, the last TN/2 the other factor's of the same outputs.
 constexpr int kLinSlabLd = 68, kLinSlabFloats = 32 * kLinSlabLd;
+__device__ __forceinline__ void lin_slab8(const float* s, float (&v)[8]) {
+  const f32x4 a = reinterpret_cast<const f32x4*>(s)[0], b = reinterpret_cast<const f32x4*>(s)[1];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+}
 // put(slab, tm, left, right): the accumulators of rows 32 tm .. and column tiles (of 32) left, right into the slab.  PLAIN: the sums alone (a backward pass: no bias, activation, residual, pre-activation).
 template <class T, int TM, int TN, bool GATED, bool PLAIN, class Put>
 __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, float* slab, int lane, long i0, long j0, int sp) {
@@ -372,28 +379,38 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, flo
     const int left = GATED ? c : 2 * c, right = GATED ? c + TN / 2 : 2 * c + 1;
     const int lr = lane / LPR;
     const long j = jc + (lane % LPR) * 8;
-    const bool in = j < cols;
+    const bool in = j + 8 <= cols, rest = !in && j < cols;     // the lane's eight columns exist; some of them do
     float b0[8], b1[8];
     if (p.splits == 1) {                                     // (PLAIN: there is none, zeros)
-      lin_bias8<T>(p, in ? j : p.rows_j, b0);
-      if (GATED) lin_bias8<T>(p, in ? p.f + j : p.rows_j, b1);
+      lin_bias8<T>(p, j < cols ? j : p.rows_j, b0);
+      if (GATED) lin_bias8<T>(p, j < cols ? p.f + j : p.rows_j, b1);
     }
 #pragma unroll
     for (int tm = 0; tm < TM; ++tm) {
       const long ir = i0 + 32 * tm + lr;                     // pass q: row ir + q RPP
-      if (!p.vec) {
-        lin_wave_sync();
-        put(slab, tm, left, right);
-        lin_wave_sync();
+      lin_u4 r[GATED ? 1 : NP][sizeof(T) / 2];
+      if (!GATED && !PLAIN && p.res && p.splits == 1) {
+#pragma unroll
+        for (int q = 0; q < (GATED ? 1 : NP); ++q)
+          if (in && ir + q * RPP < p.rows_i) {
+#pragma unroll
+            for (int h = 0; h < (int)sizeof(T) / 2; ++h)
+              r[q][h] = reinterpret_cast<const lin_u4_any*>(static_cast<const T*>(p.res) + (ir + q * RPP) * p.rows_j + j)[h];
+          }
+      }
+      lin_wave_sync();
+      put(slab, tm, left, right);
+      lin_wave_sync();
+      if (rest) {
 #pragma unroll 1
         for (int q = 0; q < NP; ++q) {
           const float* s = slab + (q * RPP + lr) * kLinSlabLd + (lane % LPR) * 8;
           const long i = ir + q * RPP;
           float v[8], u[8];
-          lin_load8<float>(s, v, true, 8);
-          if (GATED) lin_load8<float>(s + 32, u, true, 8);
+          lin_slab8(s, v);
+          if (GATED) lin_slab8(s + 32, u);
           if (p.splits > 1) {
-            const int n = cols - j < 8 ? (int)(cols - j) : 8;
+            const int n = (int)(cols - j);
             if (i < p.rows_i) {
               lin_store8<float>(part + i * p.rows_j + j, v, false, n);
               if (GATED) lin_store8<float>(part + i * p.rows_j + p.f + j, u, false, n);
@@ -404,29 +421,15 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, flo
             lin_finish8<T>(p, i, j, v, b0);
           }
         }
-        continue;
       }
-      lin_u4 r[GATED ? 1 : NP][sizeof(T) / 2];
-      if (!GATED && !PLAIN && p.res && p.splits == 1) {
-#pragma unroll
-        for (int q = 0; q < (GATED ? 1 : NP); ++q)
-          if (in && ir + q * RPP < p.rows_i) {
-#pragma unroll
-            for (int h = 0; h < (int)sizeof(T) / 2; ++h)
-              r[q][h] = reinterpret_cast<const lin_u4*>(static_cast<const T*>(p.res) + (ir + q * RPP) * p.rows_j + j)[h];
-          }
-      }
-      lin_wave_sync();
-      put(slab, tm, left, right);
-      lin_wave_sync();
 #pragma unroll
       for (int q0 = 0; q0 < NP; q0 += NG) {
         float v[NG][8], u[GATED ? NG : 1][8];
 #pragma unroll
         for (int q = 0; q < NG; ++q) {
           const float* s = slab + ((q0 + q) * RPP + lr) * kLinSlabLd + (lane % LPR) * 8;
-          lin_load8<float>(s, v[q], true, 8);
-          if (GATED) lin_load8<float>(s + 32, u[GATED ? q : 0], true, 8);
+          lin_slab8(s, v[q]);
+          if (GATED) lin_slab8(s + 32, u[GATED ? q : 0]);
         }
         if (p.splits > 1) {
 #pragma unroll
@@ -520,7 +523,7 @@ __device__ __forceinline__ void lin_join(const LinGemmArgs& p, long block) {
   const long i = t / pieces, j = (t - i * pieces) * 8;
   if (i >= p.rows_i) return;
   const int n = cols - j < 8 ? (int)(cols - j) : 8;
-  const bool vec = p.vec && n == 8;
+  const bool vec = n == 8;
   float v[8], u[8], q[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] = u[e] = 0.0f;
@@ -598,11 +601,10 @@ inline __global__ void __launch_bounds__(256) lin_pad_kernel(const LinPadArgs p)
   const long r = t / pieces;
   const int c = (int)(t - r * pieces) * 8;
   if (r >= p.rows[o]) return;
-  typedef unsigned u4_any __attribute__((ext_vector_type(4), aligned(2)));
   const unsigned short* s = p.src[o] + r * w + c;
   lin_u4 q = {0u, 0u, 0u, 0u};
   if (c + 8 <= w) {
-    q = *reinterpret_cast<const u4_any*>(s);
+    q = *reinterpret_cast<const lin_u4_any*>(s);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

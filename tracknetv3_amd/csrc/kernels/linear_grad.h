@@ -17,7 +17,7 @@ struct LinDzArgs {
   int ld_dz;
   float* part;           // [row blocks][n] / [..][2 n], or null: no bias
   long rows;
-  int n, act, rows_per_block, vec;
+  int n, act, rows_per_block;
 };
 
 template <class T, bool GATED>
@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(const LinDzArgs p) {
   const int jt = (p.n + 255) / 256, jb = blockIdx.x % jt;
   const long rb = blockIdx.x / jt;
   const int j = jb * 256 + tx * 8, n = p.n - j < 8 ? p.n - j : 8;
-  const bool vec = p.vec && n == 8;
+  const bool vec = n == 8;
   const long r0 = rb * p.rows_per_block, r1 = r0 + p.rows_per_block < p.rows ? r0 + p.rows_per_block : p.rows;
   const int ldz = GATED ? 2 * p.n : p.n;
   float s0[8], s1[8];

@@ -12,7 +12,6 @@
 
 namespace tnv3 {
 
-typedef unsigned lin_u4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <class T> __device__ __forceinline__ f32x4 lin_mfma16(lin_u4 a, lin_u4 b, f32x4 c, T) {
   return lin_mfma16(__builtin_bit_cast(lin_s8, a), __builtin_bit_cast(lin_s8, b), c, T{});
 }

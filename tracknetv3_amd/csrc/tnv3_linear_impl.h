@@ -166,7 +166,6 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   const int n2 = GATED ? 2 * n : n;
   p.a = x; p.b = w; p.rows_i = rows; p.rows_j = n2; p.kk = k; p.lda = p.ldb = k; p.splits = 1;
   p.bias = bias; p.res = res; p.out = out; p.pre = pre; p.act = act; p.f = GATED ? n : 0;
-  p.vec = n % 8 == 0;
   if (rows <= kLinFewRows) {
     const int grid = (n + 15) / 16;
     if (rows <= 16) return L.launch(lin_rows_kernel<T, 1, 16, GATED>, grid, 1024, p);
@@ -230,7 +229,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
     LinDzArgs a = {};
     a.dy = dy; a.pre = act_pass ? pre : nullptr; a.dz = act_pass ? ws + l.dz : nullptr; a.ld_dz = ldz;
     a.part = db ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
-    a.rows = rows; a.n = n; a.act = act; a.rows_per_block = (int)per; a.vec = n % 8 == 0;
+    a.rows = rows; a.n = n; a.act = act; a.rows_per_block = (int)per;
     const long blocks = (long)((n + 255) / 256) * row_blocks;
     if (int rc = lin_grid_check(blocks)) return rc;
     if (int rc = L.launch(lin_dz_kernel<T, GATED>, (int)blocks, 256, a)) return rc;
@@ -245,7 +244,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   long joins_dx = 0, joins_dw = 0;
   if (dx) {
     LinGemmArgs& p = q.dx;
-    p.a = dz; p.b = wp; p.rows_i = rows; p.rows_j = k; p.kk = n2; p.lda = ldz; p.ldb = ldk; p.out = dx; p.vec = k % 8 == 0;
+    p.a = dz; p.b = wp; p.rows_i = rows; p.rows_j = k; p.kk = n2; p.lda = ldz; p.ldb = ldk; p.out = dx;
     lin_apply(p, l.dx, reinterpret_cast<float*>(ws + l.part_dx));
     const long b = (l.dx.tiles * p.splits + 7) / 8 * 8;
     if (int rc = lin_grid_check(b)) return rc;
@@ -254,7 +253,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   }
   if (dw) {
     LinGemmArgs& p = q.dw;
-    p.a = dz; p.b = xp; p.rows_i = n2; p.rows_j = k; p.kk = rows; p.lda = ldz; p.ldb = ldk; p.out = dw; p.vec = k % 8 == 0;
+    p.a = dz; p.b = xp; p.rows_i = n2; p.rows_j = k; p.kk = rows; p.lda = ldz; p.ldb = ldk; p.out = dw;
     lin_apply(p, l.dw, reinterpret_cast<float*>(ws + l.part_dw));
     const long b = (l.dw.tiles * p.splits + 7) / 8 * 8;
     if (int rc = lin_grid_check(b)) return rc;
