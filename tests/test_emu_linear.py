@@ -92,6 +92,14 @@ def test_only_the_gradients_that_are_wanted(emu):
     assert torch.equal(dr, dy)
 
 
+def test_a_second_derivative_is_refused(emu):
+    x, w, b, r, dy = lc.make(3, 8, 6, torch.float32, residual=True)
+    w.requires_grad_()
+    for y in (ff.linear(x, w, b, r, act="silu"), ff.gated_linear(x, torch.cat([w, w]), act="silu")):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y, (w,), dy, create_graph=True)
+
+
 def test_gradients_against_differences(emu):
     """Central differences of sum(y * dy) along random directions; fp32 forward, step 2^-7: the difference's own error is about
     (step^2 |third derivative| + 2^-24 |value| / step) -- 1e-3 of the gradient's scale."""

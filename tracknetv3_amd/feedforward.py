@@ -14,7 +14,6 @@ import math
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -31,7 +30,32 @@ def _act(act):
 
 
 # (The backward passes call the ops' unchecked form: every tensor is the forward's own or has the shape and type that autograd guarantees, on the
-# device that autograd made current.)
+# device that autograd made current.  Their results would be constants to a second derivative: a graph of the backward pass is refused.)
+def _no_second_derivative():
+    if torch.is_grad_enabled():
+        raise RuntimeError("linear / gated_linear have no second derivative: backward with create_graph=True is refused")
+
+
+def _linear_grads(ctx, dy):
+    _no_second_derivative()
+    x, weight, pre = ctx.saved_tensors
+    need = ctx.needs_input_grad
+    dx = dw = db = None
+    if need[0] or need[1] or need[2]:
+        n, k = weight.shape
+        dx, dw, db = ops._linear_backward_call(False, dy if dy.is_contiguous() else dy.contiguous(), x, weight, pre, ctx.act, need, x.numel() // k, k, n,
+                                               ops._LINEAR_DTYPES[x.dtype])
+    return dx, dw, db, (dy if need[3] else None), None
+
+
+def _gated_linear_grads(ctx, dh):
+    _no_second_derivative()
+    x, weight, pre = ctx.saved_tensors
+    n2, k = weight.shape
+    return ops._linear_backward_call(True, dh if dh.is_contiguous() else dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad, x.numel() // k, k,
+                                     n2 // 2, ops._LINEAR_DTYPES[x.dtype]) + (None,)
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
@@ -40,17 +64,7 @@ class _Linear(torch.autograd.Function):
         ctx.act = act
         return y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, weight, pre = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        if need[0] or need[1] or need[2]:
-            n, k = weight.shape
-            dx, dw, db = ops._linear_backward_call(False, dy if dy.is_contiguous() else dy.contiguous(), x, weight, pre, ctx.act, need, x.numel() // k, k, n,
-                                                   ops._LINEAR_DTYPES[x.dtype])
-        return dx, dw, db, (dy if need[3] else None), None
+    backward = staticmethod(_linear_grads)
 
 
 class _GatedLinear(torch.autograd.Function):
@@ -61,13 +75,7 @@ class _GatedLinear(torch.autograd.Function):
         ctx.act = act
         return h
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh):
-        x, weight, pre = ctx.saved_tensors
-        n2, k = weight.shape
-        return ops._linear_backward_call(True, dh if dh.is_contiguous() else dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad, x.numel() // k, k,
-                                         n2 // 2, ops._LINEAR_DTYPES[x.dtype]) + (None,)
+    backward = staticmethod(_gated_linear_grads)
 
 
 def linear(x, weight, bias=None, residual=None, act="none"):
