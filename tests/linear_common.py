@@ -157,3 +157,17 @@ def check_exact(rows, k, n, dtype, gated, bias, residual, device, act="relu", se
     got = run(*cast[:4], act, gated, cast[4])
     for name, v in got.items():
         assert torch.equal(v.cpu().double(), want[name]), (name, (v.cpu().double() != want[name]).nonzero()[:4].tolist())
+    return cast, want
+
+
+def check_exact_subsets(rows, k, n, dtype, gated, device):
+    from tracknetv3_amd import ops
+    (x, w, b, _, dy), want = check_exact(rows, k, n, dtype, gated, True, False, device)
+    act = ops.ACT_RELU
+    _, pre = ops.gated_linear(x, w, b, act, want_pre=True) if gated else ops.linear(x, w, b, None, act, want_pre=True)
+    call = ops.gated_linear_backward if gated else ops.linear_backward
+    for mask in range(1, 8):
+        asked = [bool(mask & 1), bool(mask & 2), bool(mask & 4)]
+        for name, on, g in zip(("dx", "dw", "db"), asked, call(dy, x, w, pre, act, asked)):
+            assert (g is None) == (not on)
+            assert g is None or torch.equal(g.cpu().double(), want[name]), (name, asked)

@@ -92,6 +92,14 @@ def test_only_the_gradients_that_are_wanted(emu):
     assert torch.equal(dr, dy)
 
 
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(9, 40, 24), (70, 136, 130)])
+def test_each_subset_of_the_gradients(emu, rows, k, n, gated, dtype):
+    """Exact integers: whatever else is asked for, a gradient is the same."""
+    lc.check_exact_subsets(rows, k, n, dtype, gated, "cpu")
+
+
 def test_a_second_derivative_is_refused(emu):
     x, w, b, r, dy = lc.make(3, 8, 6, torch.float32, residual=True)
     w.requires_grad_()

@@ -35,6 +35,14 @@ def test_large_against_64_bits(gpu_device, gated, dtype):
 
 
 @pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(9, 40, 24), (200, 2048, 515), (1030, 520, 264), (600, 2048, 2048)])
+def test_each_subset_of_the_gradients(gpu_device, rows, k, n, gated, dtype):
+    """Exact integers: whatever else is asked for, a gradient is the same."""
+    lc.check_exact_subsets(rows, k, n, dtype, gated, gpu_device)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_views_whose_base_is_not_aligned(gpu_device, rows, dtype):
     """Contiguous tensors that start one element into their storage."""

@@ -61,14 +61,14 @@ inline void lin_set_plan(LinPlan& pl, int dtype, int tile, long rows_i, long row
   pl.k_per_split = per * 64;
   pl.part_bytes = pl.splits > 1 ? lin_pad((size_t)pl.splits * rows_i * rows_j * 4) : 0;
 }
-// the forward product: the tile and the number of parts of the contraction with the least expected time
-inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated) {
+// one product: the tile (smallest_tile or larger) and the number of parts of the contraction with the least expected time
+inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated, int smallest_tile) {
   LinPlan pl;
   double best = 0;
   int tile = kTileNormal;
   long split = 0;
   const long steps = (kk + 63) / 64;
-  for (int t = dtype == kLinF32 ? kTileNormal : kTileSmall; t <= kTileWide; ++t) {
+  for (int t = smallest_tile; t <= kTileWide; ++t) {
     const LinCost& c = lin_cost(dtype, t);
     const long tiles = lin_tiles(rows_i, rows_j, gated, c.bi, c.bj);
     for (long s : kLinSplits) {
@@ -152,7 +152,7 @@ struct LinForwardLayout { LinPlan plan; size_t x, w, part, total; };
 inline LinForwardLayout lin_forward_layout(long rows, int k, int n2, int dtype, bool gated) {
   LinForwardLayout l = {};
   if (rows <= kLinFewRows) return l;
-  l.plan = lin_plan(dtype, rows, n2, k, gated);
+  l.plan = lin_plan(dtype, rows, n2, k, gated, dtype == kLinF32 ? kTileNormal : kTileSmall);
   l.x = 0;
   l.w = l.x + lin_pad_bytes(dtype, rows, k);
   l.part = l.w + lin_pad_bytes(dtype, n2, k);
@@ -204,10 +204,13 @@ inline long lin_dz_rows(long rows, int n) {
   return per < 8 ? 8 : per;
 }
 struct LinBackwardLayout { LinPlan dx, dw; size_t dz, sums, w, x, part_dx, part_dw, total; };
-inline LinBackwardLayout lin_backward_layout(long rows, int k, int n, int act, int dtype, bool gated) {
+// for the products that are wanted (the unwanted one's plan is empty)
+inline LinBackwardLayout lin_backward_layout(long rows, int k, int n, int act, int dtype, bool gated, bool dx, bool dw) {
   const int n2 = gated ? 2 * n : n;
-  LinBackwardLayout l;
-  lin_pair_plan(l.dx, l.dw, dtype, rows, k, n2);
+  LinBackwardLayout l = {};
+  if (dx && dw) lin_pair_plan(l.dx, l.dw, dtype, rows, k, n2);
+  else if (dx) l.dx = lin_plan(dtype, rows, k, n2, false, kTileNormal);
+  else if (dw) l.dw = lin_plan(dtype, n2, k, rows, false, kTileNormal);
   const long per = lin_dz_rows(rows, n);
   l.dz = 0;
   l.sums = l.dz + (gated || act != kActNone ? lin_pad((size_t)rows * lin_ld(dtype, n2) * lin_size(dtype)) : lin_pad_bytes(dtype, rows, n2));
@@ -263,13 +266,14 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   q.sums = reinterpret_cast<const float*>(ws + l.sums); q.db = db; q.sum_rows = (int)row_blocks; q.sum_cols = n2;
   const long grid = (long)q.blocks_dx + q.blocks_dw + (db ? (n2 + 127) / 128 : 0);
   if (grid == 0) return 0;
+  const int tile = dx ? l.dx.tile : (dw ? l.dw.tile : kTileNormal);
   if (int rc = lin_grid_check(grid > joins_dx + joins_dw ? grid : joins_dx + joins_dw)) return rc;
   int rc;
   if constexpr (sizeof(T) == 2) {
-    if (l.dx.tile == kTileWide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
+    if (tile == kTileWide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
     else rc = L.launch(lin_dma_pair_kernel<LinD128, T>, (int)grid, LinD128::NT, q);
   } else {
-    if (l.dx.tile == kTileWide) rc = L.launch(lin_split_pair_kernel<LinF256>, (int)grid, LinF256::NT, q);
+    if (tile == kTileWide) rc = L.launch(lin_split_pair_kernel<LinF256>, (int)grid, LinF256::NT, q);
     else rc = L.launch(lin_split_pair_kernel<LinF128>, (int)grid, LinF128::NT, q);
   }
   if (rc || joins_dx + joins_dw == 0) return rc;
@@ -296,7 +300,12 @@ inline size_t lin_forward_workspace_bytes(long rows, int k, int n, int dtype, bo
 }
 inline size_t lin_backward_workspace_bytes(long rows, int k, int n, int act, int dtype, bool gated) {
   if (lin_check("workspace", rows, k, n, act, dtype, gated)) return 0;
-  return lin_backward_layout(rows, k, n, act, dtype, gated).total;
+  size_t most = 0;
+  for (int want = 1; want < 4; ++want) {
+    const size_t t = lin_backward_layout(rows, k, n, act, dtype, gated, want & 1, want & 2).total;
+    most = t > most ? t : most;
+  }
+  return most;
 }
 
 template <bool GATED, class Launcher>
@@ -323,7 +332,7 @@ int lin_backward_impl(Launcher& L, const void* dy, const void* x, const void* w,
   if (!dy || (dx && !w) || (dw && !x)) TNV3_FAIL(-1, "%s: null tensor", what);
   if ((GATED || act != kActNone) && !pre) TNV3_FAIL(-1, "%s: the forward's pre-activation is required", what);
   if (!lin_all_aligned(dy, x, w, pre, dx, dw, db, ws)) TNV3_FAIL(-1, "%s: tensors must be 16-byte aligned", what);
-  const LinBackwardLayout l = lin_backward_layout(rows, k, n, act, dtype, GATED);
+  const LinBackwardLayout l = lin_backward_layout(rows, k, n, act, dtype, GATED, dx != nullptr, dw != nullptr);
   if (!ws || ws_bytes < l.total) TNV3_FAIL(-1, "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, l.total);
   char* wsc = static_cast<char*>(ws);
   switch (dtype) {
