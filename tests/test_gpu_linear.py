@@ -196,3 +196,49 @@ def test_training_step_of_the_block_follows_the_oracle(gpu_device):
     for k, v in block.named_parameters():
         # three updates of lr * gradient (|gradient| < 1 here), each within fp32's 2^-18 of the gradient's norm, plus the parameter's rounding
         assert (v.cpu().double() - ref[k]).abs().max() <= 2.0 ** -20, k
+
+
+def _signs(shape, keep, device, gen, dtype):
+    """-1, 0, 1 with about `keep` nonzero; exact in every type."""
+    r = torch.rand(shape, generator=gen, device=device)
+    return ((r < keep / 2).to(dtype) - (r > 1 - keep / 2).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_operands_beyond_2_to_the_32_bytes_and_elements(gpu_device, dtype):
+    """Long batches and large weights: the offsets pass 32 bits.  Integer operands, so the compared parts are equal."""
+    gen = torch.Generator(device=gpu_device).manual_seed(1)
+    # rows x k beyond 2^31 elements (2^32 bytes in bf16): x, dx and the contraction of dW are long
+    rows, k, n = (1 << 19) + 131, 4160, 72
+    x = _signs((rows, k), 0.002, gpu_device, gen, dtype)
+    w = _signs((n, k), 0.1, gpu_device, gen, dtype)
+    dy = _signs((rows, n), 0.002, gpu_device, gen, dtype)
+    y = ops.linear(x, w)
+    dx, dw, db = ops.linear_backward(dy, x, w)
+    for part in (slice(0, 300), slice(rows // 2, rows // 2 + 300), slice(rows - 300, rows)):
+        assert torch.equal(y[part].float(), x[part].float() @ w.float().t())
+        assert torch.equal(dx[part].float(), dy[part].float() @ w.float())
+    want = torch.zeros(n, k, device=gpu_device)
+    for at in range(0, rows, 1 << 16):
+        want += dy[at:at + (1 << 16)].float().t() @ x[at:at + (1 << 16)].float()
+    assert want.abs().max() <= 256 and torch.equal(dw.float(), want)
+    assert torch.equal(db.float(), dy.float().sum(0).to(dtype).float())
+    del x, y, dx, dy
+    # a weight beyond 2^31 elements, few and more rows; its gradient is as large
+    n, k = 1 << 19, 4168
+    w = _signs((n, k), 0.003, gpu_device, gen, dtype)
+    for rows in (3, 70):
+        x = _signs((rows, k), 0.5, gpu_device, gen, dtype)
+        y, h = ops.linear(x, w), ops.gated_linear(x, w, act=ops.ACT_RELU)
+        for part in (slice(0, 300), slice(n // 2 - 300, n // 2), slice(n - 300, n)):
+            assert torch.equal(y[:, part].float(), x.float() @ w[part].float().t())
+        last = slice(n // 2 - 300, n // 2)
+        g, u = (x.float() @ w[r].float().t() for r in (last, slice(n - 300, n)))
+        assert torch.equal(h[:, last].float(), torch.relu(g) * u)
+    dy = _signs((70, n), 0.001, gpu_device, gen, dtype)
+    dx, dw, _ = ops.linear_backward(dy, x, w, want=(True, True, False))
+    assert torch.equal(dw[-300:].float(), dy[:, -300:].float().t() @ x.float())
+    want = torch.zeros(70, k, device=gpu_device)
+    for at in range(0, n, 1 << 16):
+        want += dy[:, at:at + (1 << 16)].float() @ w[at:at + (1 << 16)].float()
+    assert want.abs().max() <= 256 and torch.equal(dx.float(), want)
