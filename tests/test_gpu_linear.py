@@ -1,4 +1,6 @@
 """GPU: the position-wise layers on the MI355X through the public entry points -- every kernel variant's sizes, alignments, streams, graph replay."""
+import gc
+
 import pytest
 import torch
 
@@ -140,6 +142,32 @@ def test_block_captured_and_replayed(gpu_device, rows):
         got = [t.clone() for t in captured]
         for a, b in zip(got, step()):
             assert torch.equal(a, b), i
+
+
+def test_captured_backward_beside_an_eager_graph_of_the_same_leaves_is_refused(gpu_device):
+    """The refusal comes before anything of the backward pass is launched; afterwards eager and captured steps work as before."""
+    block = ff.GatedFeedForward(64, 96).to(gpu_device)
+    params = list(block.parameters())
+    x = torch.randn(20, 64, device=gpu_device)
+    dy = torch.randn(20, 64, device=gpu_device)
+    eager = block(x)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            y = block(x)
+            torch.autograd.grad(y, params, dy)
+    del graph, y
+    want = torch.autograd.grad(eager, params, dy)
+    del eager
+    gc.collect()                       # the exception's frames hold the refused graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(block(x), params, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
 
 
 def test_two_graphs_keep_their_own_workspaces(gpu_device):

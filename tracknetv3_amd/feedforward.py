@@ -9,6 +9,8 @@ fp32, bf16 or fp16.  `x` is (..., k) with any leading shape, one position per ro
     y = block(x)                                  # x + W_out (silu(W_gate x) * W_up x)
 
 The pre-activation is kept for the backward pass -- linear's in the tensors' type, gated_linear's in fp32 -- and sums are fp32.
+A captured backward pass needs that no eager graph over the same parameters from the default stream is alive (it is refused otherwise): drop the
+outputs of earlier steps, or run them on a side stream.
 """
 import math
 
@@ -36,9 +38,29 @@ def _no_second_derivative():
         raise RuntimeError("linear / gated_linear have no second derivative: backward with create_graph=True is refused")
 
 
+# A leaf's gradient accumulator belongs to the stream on which the first graph over the leaf was recorded and lives as long as any graph over it.  If
+# that is the default stream, a backward pass captured on another would have to make the default stream wait inside the capture, which the runtime
+# answers by ending the process: such a call is refused, before anything of the backward pass is launched.
+def _record_stream_of_accumulators(ctx, x):
+    if x.is_cuda:
+        stream = torch._C._cuda_getCurrentRawStream(x.get_device())
+        for node, _ in ctx.next_functions:
+            if node is not None:
+                node.metadata.setdefault("tnv3_stream", stream)
+
+
+def _capturable(ctx, x):
+    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+        for node, _ in ctx.next_functions:
+            if node is not None and node.metadata.get("tnv3_stream") == 0:
+                raise RuntimeError("linear / gated_linear: this backward pass is being captured while an eager graph of the same tensors, recorded on the "
+                                   "default stream, is alive: drop its outputs first, or run it on a side stream")
+
+
 def _linear_grads(ctx, dy):
     _no_second_derivative()
     x, weight, pre = ctx.saved_tensors
+    _capturable(ctx, x)
     need = ctx.needs_input_grad
     dx = dw = db = None
     if need[0] or need[1] or need[2]:
@@ -51,6 +73,7 @@ def _linear_grads(ctx, dy):
 def _gated_linear_grads(ctx, dh):
     _no_second_derivative()
     x, weight, pre = ctx.saved_tensors
+    _capturable(ctx, x)
     n2, k = weight.shape
     return ops._linear_backward_call(True, dh if dh.is_contiguous() else dh.contiguous(), x, weight, pre, ctx.act, ctx.needs_input_grad, x.numel() // k, k,
                                      n2 // 2, ops._LINEAR_DTYPES[x.dtype]) + (None,)
@@ -62,6 +85,7 @@ class _Linear(torch.autograd.Function):
         y, pre = ops.linear(x, weight, bias, residual, act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
+        _record_stream_of_accumulators(ctx, x)
         return y
 
     backward = staticmethod(_linear_grads)
@@ -73,6 +97,7 @@ class _GatedLinear(torch.autograd.Function):
         h, pre = ops.gated_linear(x, weight, bias, act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
+        _record_stream_of_accumulators(ctx, x)
         return h
 
     backward = staticmethod(_gated_linear_grads)
