@@ -171,3 +171,35 @@ def check_exact_subsets(rows, k, n, dtype, gated, device):
         for name, on, g in zip(("dx", "dw", "db"), asked, call(dy, x, w, pre, act, asked)):
             assert (g is None) == (not on)
             assert g is None or torch.equal(g.cpu().double(), want[name]), (name, asked)
+
+
+def check_nan_stays_in_place(rows, k, n, dtype, gated, device, seed=0):
+    """A NaN row of x, of dy or of the weight reaches the results that it enters and leaves every other one as it was, to the bit: nothing of a
+    neighbouring row is read into a product, nothing is multiplied by a zero that stands for "not there"."""
+    act = "silu"
+    x, w, b, _, dy = make(rows, k, n, dtype, gated, True, False, seed, device)
+    clean = run(x, w, b, None, act, gated, dy)
+    for r in sorted({0, rows // 2, rows - 1}):
+        others = torch.arange(rows, device=device) != r
+        bad = x.clone()
+        bad[r] = float("nan")
+        got = run(bad, w, b, None, act, gated, dy)
+        assert torch.isnan(got["y"][r]).all() and torch.isnan(got["dx"][r]).all() and torch.isnan(got["dw"]).all()
+        assert torch.equal(got["y"][others], clean["y"][others]) and torch.equal(got["dx"][others], clean["dx"][others]), ("x", r)
+        bad = dy.clone()
+        bad[r] = float("nan")
+        got = run(x, w, b, None, act, gated, bad)
+        assert torch.equal(got["y"], clean["y"]) and torch.equal(got["dx"][others], clean["dx"][others]), ("dy", r)
+        assert torch.isnan(got["dx"][r]).all() and torch.isnan(got["dw"]).all() and torch.isnan(got["db"]).all()
+    wide = w.shape[0]
+    for j in sorted({0, n - 1, wide - 1}):
+        others = torch.arange(wide, device=device) != j
+        if gated:
+            others = others & (torch.arange(wide, device=device) % n != j % n)        # the pair's other row sees the NaN in its factor
+        bad = w.clone()
+        bad[j] = float("nan")
+        got = run(x, bad, b, None, act, gated, dy)
+        cols = torch.arange(n, device=device) != j % n
+        assert torch.isnan(got["y"][:, j % n]).all() and torch.equal(got["y"][:, cols], clean["y"][:, cols]), ("w", j)
+        assert torch.isnan(got["dx"]).all() and torch.isnan(got["dw"][j % n]).all()         # (gated: act'(g) u, whichever is NaN)
+        assert torch.equal(got["dw"][others], clean["dw"][others]) and torch.equal(got["db"][others], clean["db"][others]), ("w", j)

@@ -70,6 +70,13 @@ def test_fp32_keeps_infinities_and_nan_where_they_belong(emu, monkeypatch, cus):
     assert torch.equal(torch.sign(y[torch.isinf(want)]), torch.sign(want[torch.isinf(want)]))
 
 
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(1, 5, 3), (6, 70, 9), (19, 33, 17), (70, 67, 35), (66, 136, 72)])
+def test_nan_stays_in_its_row(emu, rows, k, n, gated, dtype):
+    lc.check_nan_stays_in_place(rows, k, n, dtype, gated, "cpu")
+
+
 def test_zero_rows(emu):
     x = torch.zeros(0, 12, requires_grad=True)
     w = torch.randn(10, 12, requires_grad=True)

@@ -79,6 +79,13 @@ def test_fp32_keeps_infinities_and_nan_where_they_belong(gpu_device):
 
 
 @pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(1, 5, 3), (6, 70, 9), (33, 513, 40), (70, 67, 35), (130, 72, 140), (300, 1001, 333), (700, 2050, 600)])
+def test_nan_stays_in_its_row(gpu_device, rows, k, n, gated, dtype):
+    lc.check_nan_stays_in_place(rows, k, n, dtype, gated, gpu_device)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
 def test_rows_behind_the_last_stay_as_they_were(gpu_device, dtype):
     """Outputs are written up to their last element and not beyond, at sizes that end inside a tile, a vector and a row block."""
     lib, p = ops._lib.load(), ops._lib.ptr

@@ -1,12 +1,13 @@
 // linear_common.h -- what the position-wise products share (linear, gated_linear and their backward passes): element types, the
-// MFMA 32x32x16 fragments, the activations with their derivatives, and the write-out of a workgroup's tile.
+// MFMA fragments, the activations with their derivatives, and the write-out of a workgroup's tile.
 //
 // Every product is C(i, j) = sum_k A(i, k) B(j, k) with fp32 accumulators:
 //   forward          i = row m of x,      j = output column n,  k = input column:  A = x,   B = W        both k-contiguous
 //   gradient of x    i = row m,           j = input column,     k = output column: A = dz,  B = W^T      B strided in k
 //   gradient of W    i = output column,   j = input column,     k = row m:         A = dz^T, B = x^T     both strided in k
-// MFMA 32x32x16 (16-bit operands): lane l supplies A[l & 31][8 (l >> 5) + 0..7] and B[l & 31][the same k]; accumulator register r of lane l
-// is C[(r & 3) + 8 (r >> 2) + 4 (l >> 5)][l & 31].
+// MFMA 32x32x16 (the fp32 products' planes): lane l supplies A[l & 31][8 (l >> 5) + 0..7] and B[l & 31][the same k]; accumulator register r of lane l
+// is C[(r & 3) + 8 (r >> 2) + 4 (l >> 5)][l & 31].  16x16x32 (16-bit tensors): A[l & 15][8 (l >> 4) + 0..7], B likewise; register r of lane l is
+// C[4 (l >> 4) + r][l & 15].
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
@@ -198,7 +199,7 @@ template <bool FAST> __device__ __forceinline__ void lin_act_grad1(float z, int 
   switch (act) {
     case kActLeaky: a = z > 0.0f ? z : 0.01f * z; d = z > 0.0f ? 1.0f : 0.01f; return;
     case kActSigmoid: { const float s = lin_sigmoid<FAST>(zc); a = s; d = s * (1.0f - s); return; }
-    case kActRelu: a = z > 0.0f ? z : (z != z ? z : 0.0f); d = z > 0.0f ? 1.0f : 0.0f; return;
+    case kActRelu: a = z > 0.0f ? z : (z != z ? z : 0.0f); d = z <= 0.0f ? 0.0f : 1.0f; return;
     case kActSilu: { const float s = lin_sigmoid<FAST>(zc); a = z * s; d = s * (1.0f + zc * (1.0f - s)); return; }
     case kActGelu: { const float p = lin_phi<FAST>(zc); a = z * p; d = p + 0.39894228040143268f * zc * lin_exp<FAST>(-0.5f * zc * zc); return; }
     case kActGeluTanh: {

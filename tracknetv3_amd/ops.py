@@ -1208,6 +1208,8 @@ def _linear_workspace(lib, entry, x, *sizes):
         key = (entry, x.get_device()) + sizes
         need = _LINEAR_WORKSPACE.get(key)
         if need is None:
+            if len(_LINEAR_WORKSPACE) >= 4096:          # batches of ever new sizes
+                _LINEAR_WORKSPACE.clear()
             need = _LINEAR_WORKSPACE[key] = getattr(lib, entry)(*sizes)
     return (torch.empty((need + 7) // 8, dtype=torch.int64, device=x.device), need) if need else (None, 0)
 
