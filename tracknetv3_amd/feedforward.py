@@ -50,7 +50,7 @@ def _record_stream_of_accumulators(ctx, x):
 
 
 def _capturable(ctx, x):
-    if x.is_cuda and torch.cuda.is_current_stream_capturing():
+    if x.is_cuda and torch._C._cuda_isCurrentStreamCapturing():
         for node, _ in ctx.next_functions:
             if node is not None and node.metadata.get("tnv3_stream") == 0:
                 raise RuntimeError("linear / gated_linear: this backward pass is being captured while an eager graph of the same tensors, recorded on the "

@@ -1211,7 +1211,7 @@ def _linear_workspace(lib, entry, x, *sizes):
             if len(_LINEAR_WORKSPACE) >= 4096:          # batches of ever new sizes
                 _LINEAR_WORKSPACE.clear()
             need = _LINEAR_WORKSPACE[key] = getattr(lib, entry)(*sizes)
-    return (torch.empty((need + 7) // 8, dtype=torch.int64, device=x.device), need) if need else (None, 0)
+    return (x.new_empty((need + 3) // x.element_size()), need) if need else (None, 0)
 
 
 def _address(t):
@@ -1235,7 +1235,7 @@ def linear(x, weight, bias=None, residual=None, act=ACT_NONE, want_pre=False):
     shape = x.shape[:-1] + (n,)
     if residual is not None:
         _linear_tensor("linear", "residual", residual, x, x.dtype, shape)
-    y = torch.empty(shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(shape)
     pre = torch.empty_like(y) if want_pre and act != ACT_NONE else None
     if rows:
         x, weight, bias, residual = _boundary(x), _boundary(weight), _boundary(bias), _boundary(residual)
@@ -1250,8 +1250,8 @@ def gated_linear(x, weight, bias=None, act=ACT_SILU, want_pre=False):
     want_pre: returns (h, pre) -- the fp32 pre-activations (..., 2 n) that gated_linear_backward takes."""
     lib = _lib.load()
     rows, k, n, code = _linear_check("gated_linear", x, weight, bias, act, True)
-    h = torch.empty(x.shape[:-1] + (n,), dtype=x.dtype, device=x.device)
-    pre = torch.empty(x.shape[:-1] + (2 * n,), dtype=torch.float32, device=x.device) if want_pre else None
+    h = x.new_empty(x.shape[:-1] + (n,))
+    pre = x.new_empty(x.shape[:-1] + (2 * n,), dtype=torch.float32) if want_pre else None
     if rows:
         x, weight, bias = _boundary(x), _boundary(weight), _boundary(bias)
         ws, need = _linear_workspace(lib, "tnv3_gated_linear_forward_workspace_bytes", x, rows, k, n, code)
@@ -1281,7 +1281,7 @@ def _linear_backward_call(gated, dy, x, weight, pre, act, want, rows, k, n, code
     dy, x, weight, pre = _boundary(dy), _boundary(x), _boundary(weight), _boundary(pre)
     dx = torch.empty_like(x) if want[0] else None
     dw = torch.empty_like(weight) if want[1] else None
-    db = torch.empty(n2, dtype=x.dtype, device=x.device) if want[2] else None
+    db = x.new_empty(n2) if want[2] else None
     ws, need = _linear_workspace(lib, "tnv3_gated_linear_backward_workspace_bytes" if gated else "tnv3_linear_backward_workspace_bytes", x, rows, k, n,
                                  act, code)
     call = lib.tnv3_gated_linear_backward if gated else lib.tnv3_linear_backward
