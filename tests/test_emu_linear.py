@@ -199,3 +199,15 @@ def test_refusals(emu):
     assert fwd(xp=p(off)) != 0 and fwd() == 0
     assert torch.equal(ops.linear(off + 1, torch.ones(6, 8)), torch.full((4, 6), 8.0))
     assert torch.equal(ops.linear(off, w), torch.zeros(4, 6))                                                                # the op copies such a view
+
+
+def test_a_launch_that_counts_more_than_32_bits_of_work_items_is_refused(emu):
+    """2^30 rows of 33 elements: the copy into whole pieces would be 2^24 and more workgroups of 256; refused before anything is launched, so the
+    tensors and the workspace need not be there in full."""
+    lib, p = _lib.load(), _lib.ptr
+    t = torch.zeros(64, dtype=torch.bfloat16)
+    rows = 1 << 30
+    need = lib.tnv3_linear_forward_workspace_bytes(rows, 33, 8, 1)
+    assert need > rows * 80 - 1
+    assert lib.tnv3_linear_forward(p(t), p(t), None, None, p(t), None, p(t), need, rows, 33, 8, 0, 1, None) != 0
+    assert b"more than one launch takes" in lib.tnv3_last_error()

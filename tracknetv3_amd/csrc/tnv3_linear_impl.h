@@ -117,8 +117,9 @@ inline void lin_apply(LinGemmArgs& p, const LinPlan& pl, float* part) {
   p.part = part;
 }
 inline long lin_join_blocks(const LinGemmArgs& p, bool gated) { return (p.rows_i * (((gated ? (long)p.f : p.rows_j) + 7) / 8) + 255) / 256; }
-inline int lin_grid_check(long blocks) {
-  if (blocks >= (1l << 31)) TNV3_FAIL(-1, "linear: %ld workgroups are more than one launch takes", blocks);
+// a launch counts its work-items in 32 bits
+inline int lin_grid_check(long blocks, int threads) {
+  if (blocks >= (1l << 32) / threads) TNV3_FAIL(-1, "linear: %ld workgroups of %d are more than one launch takes", blocks, threads);
   return 0;
 }
 // 16-bit rows that are no whole 16-byte pieces are copied into the workspace
@@ -141,7 +142,7 @@ struct LinPadder {
   }
   template <class Launcher> int launch(Launcher& L) {
     if (!count) return 0;
-    if (int rc = lin_grid_check(blocks)) return rc;
+    if (int rc = lin_grid_check(blocks, 256)) return rc;
     return L.launch(lin_pad_kernel, (int)blocks, 256, a);
   }
 };
@@ -177,8 +178,9 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   p.b = pad.add(dtype, w, n2, k, ws + l.w);
   p.lda = p.ldb = lin_ld(dtype, k);
   lin_apply(p, l.plan, reinterpret_cast<float*>(ws + l.part));
-  const long grid = l.plan.tiles * p.splits, join = lin_join_blocks(p, GATED);
-  if (int rc = lin_grid_check(grid > join ? grid : join)) return rc;
+  const long grid = l.plan.tiles * p.splits, join = p.splits > 1 ? lin_join_blocks(p, GATED) : 0;
+  if (int rc = lin_grid_check(grid, 512)) return rc;
+  if (int rc = lin_grid_check(join, 256)) return rc;
   if (int rc = pad.launch(L)) return rc;
   int rc;
   if constexpr (sizeof(T) == 2) {
@@ -234,7 +236,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
     a.part = db ? reinterpret_cast<float*>(ws + l.sums) : nullptr;
     a.rows = rows; a.n = n; a.act = act; a.rows_per_block = (int)per;
     const long blocks = (long)((n + 255) / 256) * row_blocks;
-    if (int rc = lin_grid_check(blocks)) return rc;
+    if (int rc = lin_grid_check(blocks, 256)) return rc;
     if (int rc = L.launch(lin_dz_kernel<T, GATED>, (int)blocks, 256, a)) return rc;
   }
   LinPadder pad, pad_dy;
@@ -250,7 +252,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
     p.a = dz; p.b = wp; p.rows_i = rows; p.rows_j = k; p.kk = n2; p.lda = ldz; p.ldb = ldk; p.out = dx;
     lin_apply(p, l.dx, reinterpret_cast<float*>(ws + l.part_dx));
     const long b = (l.dx.tiles * p.splits + 7) / 8 * 8;
-    if (int rc = lin_grid_check(b)) return rc;
+    if (int rc = lin_grid_check(b, 512)) return rc;
     q.blocks_dx = (int)b;
     if (p.splits > 1) joins_dx = lin_join_blocks(p, false);
   }
@@ -259,7 +261,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
     p.a = dz; p.b = xp; p.rows_i = n2; p.rows_j = k; p.kk = rows; p.lda = ldz; p.ldb = ldk; p.out = dw;
     lin_apply(p, l.dw, reinterpret_cast<float*>(ws + l.part_dw));
     const long b = (l.dw.tiles * p.splits + 7) / 8 * 8;
-    if (int rc = lin_grid_check(b)) return rc;
+    if (int rc = lin_grid_check(b, 512)) return rc;
     q.blocks_dw = (int)b;
     if (p.splits > 1) joins_dw = lin_join_blocks(p, false);
   }
@@ -267,7 +269,8 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   const long grid = (long)q.blocks_dx + q.blocks_dw + (db ? (n2 + 127) / 128 : 0);
   if (grid == 0) return 0;
   const int tile = dx ? l.dx.tile : (dw ? l.dw.tile : kTileNormal);
-  if (int rc = lin_grid_check(grid > joins_dx + joins_dw ? grid : joins_dx + joins_dw)) return rc;
+  if (int rc = lin_grid_check(grid, 512)) return rc;
+  if (int rc = lin_grid_check(joins_dx + joins_dw, 256)) return rc;
   int rc;
   if constexpr (sizeof(T) == 2) {
     if (tile == kTileWide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
