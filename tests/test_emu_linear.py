@@ -41,6 +41,20 @@ def test_split_contraction_joins_all_parts(emu, monkeypatch):
 
 
 @pytest.mark.parametrize("lazy", ["0", "1"])
+@pytest.mark.parametrize("rows,k,n", [(17, 4104, 40), (40, 2104, 24), (64, 2100, 72), (64, 2104, 72)])
+def test_few_rows_of_a_long_contraction(emu, monkeypatch, rows, k, n, lazy):
+    """Up to 64 rows on tiles: steps of fewer elements than stages, of as many and of more."""
+    monkeypatch.setenv("TNV3_EMU_LAZY_DMA", lazy)
+    # parts to join: not the few-rows kernel, which wins where the tiles would need a copy into whole pieces
+    assert (_lib.load().tnv3_linear_forward_workspace_bytes(rows, k, n, 1) > 0) == (k % 8 == 0)
+    for cus in ("256", "8", "1"):
+        monkeypatch.setenv("TNV3_EMU_CUS", cus)
+        for dtype in lc.DTYPES:
+            lc.check_exact(rows, k, n, dtype, False, True, True, "cpu")
+        lc.check_exact(rows, k, n, torch.bfloat16, True, True, False, "cpu")
+
+
+@pytest.mark.parametrize("lazy", ["0", "1"])
 @pytest.mark.parametrize("cus", ["1", "256"])
 def test_direct_loads_land_before_they_are_read(emu, monkeypatch, cus, lazy):
     """16-bit operands that move by direct loads: pieces landing as early or as late as the program's waits allow; one CU makes the wide tiles

@@ -23,6 +23,15 @@ def test_exact_integers(gpu_device, rows, k, n, gated, dtype):
 
 
 @pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,k,n", [(17, 8192, 40), (33, 8200, 1000), (40, 2104, 24), (64, 4096, 4096), (65, 128, 4096), (100, 192, 520), (200, 4096, 2056),
+                                      (400, 2048, 4096), (260, 320, 8192)])
+def test_exact_integers_at_some_hundred_rows(gpu_device, rows, k, n, gated, dtype):
+    """Around the border between the few-rows kernel and tiles, contractions of fewer steps than LDS stages and of many, one and two workgroups per CU."""
+    lc.check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device=gpu_device, seed=rows + k)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
 @pytest.mark.parametrize("gated,act", [(False, a) for a in lc.ACTS] + [(True, a) for a in lc.ACTS if a != "none"])
 @pytest.mark.parametrize("rows,k,n", [(1, 96, 40), (9, 40, 24), (150, 264, 136)])
 def test_activations_and_gradients(gpu_device, rows, k, n, act, gated, dtype):

@@ -10,13 +10,14 @@
 
 namespace tnv3 {
 
-template <int TM_, int TN_, int WM_, int WN_>
+template <int TM_, int TN_, int WM_, int WN_, int NS_ = 2>
 struct LinDmaCfg {
   static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
+  static constexpr int NS = NS_;                                                // LDS stages: NS - 1 steps of loads are in flight
   static constexpr int NW = WM * WN, NT = NW * 64, BI = TM * 32 * WM, BJ = TN * 32 * WN, BK = 64;
   static constexpr int STAGE = (BI + BJ) * BK;                                  // 16-bit elements
   static constexpr int SLABS = NW * kLinSlabFloats * 2;
-  static constexpr int LDS = 2 * STAGE > SLABS ? 2 * STAGE : SLABS;
+  static constexpr int LDS = NS * STAGE > SLABS ? NS * STAGE : SLABS;
 };
 
 // One operand's direct loads: a wave moves ROWS / 8 / NW pieces of 1 KB per step (64 lanes x 16 bytes, consecutive in LDS; the lane picks the chunk
@@ -64,16 +65,18 @@ struct LinDma {
   }
 };
 
-__device__ __forceinline__ void lin_dma_sync() {
+// this wave's loads but for the newest LEAVE have landed, its fragments are in registers
+template <int LEAVE> __device__ __forceinline__ void lin_dma_sync() {
+  static_assert(LEAVE < 64, "vmcnt's range");
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0): this wave's loads have landed, its fragments are in registers
+  __builtin_amdgcn_s_waitcnt(0x0070 | (LEAVE & 15) | (LEAVE >> 4) << 14);              // vmcnt(LEAVE) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 }
 
 template <class Cfg, class T, bool KSA, bool KSB, bool GATED>
 __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block, unsigned short* lds) {
-  constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, STAGE = Cfg::STAGE, Q = BK / 16;
+  constexpr int TM = Cfg::TM, TN = Cfg::TN, BI = Cfg::BI, BJ = Cfg::BJ, BK = Cfg::BK, STAGE = Cfg::STAGE, NS = Cfg::NS, Q = BK / 16;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wi = wave / Cfg::WN, wj = wave % Cfg::WN;
   int ti, tj, sp;
@@ -158,7 +161,7 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       }
   };
   // From one barrier to the next: the last quarter's products of the step before (its fragments are in registers), then three quarters of this one.
-  // Every read is from `rd`, every direct load goes to `wr`, the other stage.  (The qualifiers say so to the compiler, which otherwise lets each
+  // Every read is from `rd`, every direct load goes to `wr`, the stage that was read before.  (The qualifiers say so to the compiler, which otherwise lets each
   // transposing read wait for all loads in flight.  The fences keep the reads ahead of the products: left alone, the scheduler puts each read right
   // in front of its use.)
   auto step = [&](const unsigned short* __restrict__ rd, unsigned short* __restrict__ wr, auto first) {
@@ -178,23 +181,29 @@ __device__ __forceinline__ void lin_dma_product(const LinGemmArgs& p, int block,
       products(q, wr, q == 0 ? PQ : -1);
       if (q == 1) begin();                      // the next step's descriptors (beyond the last step: zeros into a stage that is not read)
     }
-    lin_dma_sync();
+    lin_dma_sync<(NS - 2) * NP>();
   };
   if (steps > 0) {
-    begin();
 #pragma unroll
-    for (int i = 0; i < NP; ++i) piece(lds, i);
-    begin();
-    lin_dma_sync();
-    // (two steps per turn: the stages' addresses are constants then, nothing is computed between the barrier and the first reads)
-    step(lds, lds + STAGE, LinFlag<true>{});
-    int s = 1;
-    for (; s + 1 < steps; s += 2) {
-      step(lds + STAGE, lds, LinFlag<false>{});
-      step(lds, lds + STAGE, LinFlag<false>{});
+    for (int st = 0; st < NS - 1; ++st) {
+      begin();
+#pragma unroll
+      for (int i = 0; i < NP; ++i) piece(lds + st * STAGE, i);
     }
-    if (s < steps) step(lds + STAGE, lds, LinFlag<false>{});
+    begin();
+    lin_dma_sync<(NS - 2) * NP>();
+    // (NS steps per turn: the stages' addresses are constants then, nothing is computed between the barrier and the first reads)
+    step(lds, lds + (NS - 1) * STAGE, LinFlag<true>{});
+    int s = 1;
+    for (; s + NS - 1 < steps; s += NS) {
+#pragma unroll
+      for (int c = 0; c < NS; ++c) step(lds + (c + 1) % NS * STAGE, lds + c * STAGE, LinFlag<false>{});
+    }
+#pragma unroll
+    for (int c = 0; c < NS - 1; ++c)
+      if (s + c < steps) step(lds + (c + 1) % NS * STAGE, lds + c * STAGE, LinFlag<false>{});
     products(3, lds, -1);
+    if (NS > 2) lin_dma_sync<0>();                // the stages become the write-out's slabs
   }
   auto put = [&](float* slab, int tm, int left, int right) { lin_put16(acc, slab, tm, left, right, lane); };
   lin_write_out<T, TM, TN, GATED, KSB>(p, put, reinterpret_cast<float*>(lds) + wave * kLinSlabFloats, lane, i0 + wi * TM * 32,

@@ -11,7 +11,10 @@ namespace tnv3 {
 
 using LinD256 = LinDmaCfg<2, 4, 4, 2>;          // 256 x 256, eight waves of 64 x 128: one workgroup per CU
 using LinD128 = LinDmaCfg<2, 2, 2, 2>;          // 128 x 128, four waves of 64 x 64: two workgroups per CU
-using LinD64 = LinDmaCfg<1, 2, 2, 1>;           // 64 x 64, two waves of 32 x 64: forward products of few tiles
+// forward products of few tiles, whose operands come from memory rather than a cache: four LDS stages, so that three steps' loads are in flight (two
+// stages: 200 x 4096 -> 8192 in bf16 51 us instead of 31, 200 x 4096 -> 4096 32 instead of 22)
+using LinD128x4 = LinDmaCfg<2, 2, 2, 2, 4>;     // 128 x 128, one workgroup per CU
+using LinD64 = LinDmaCfg<1, 2, 2, 1, 4>;        // 64 x 64, two waves of 32 x 64, two workgroups per CU
 using LinF256 = LinSplitCfg<2, 2, 4, 2>;        // fp32: 256 x 128, eight waves of 64 x 64, one workgroup per CU (144 KB of LDS)
 using LinF128 = LinSplitCfg<1, 2, 4, 1>;        // fp32: 128 x 64, four waves of 32 x 64, two workgroups per CU
 
@@ -22,24 +25,26 @@ inline size_t lin_pad(size_t b) { return (b + 255) & ~(size_t)255; }
 inline int lin_size(int dtype) { return dtype == kLinF32 ? 4 : 2; }
 
 // One product's tiling.  Sizes and type decide, never the pointers, so that the workspace queries and the launches agree.
-enum { kTileSmall = 0, kTileNormal = 1, kTileWide = 2 };
+enum { kTileSmall = 0, kTileDeep = 1, kTileNormal = 2, kTileWide = 3 };
 struct LinPlan {
   int tile, bi, bj, splits;
   long k_per_split, tiles;
   size_t part_bytes;
+  double time;              // expected, us
 };
 inline long lin_tiles(long rows_i, long rows_j, bool gated, int bi, int bj) {
   return ((rows_i + bi - 1) / bi) * (gated ? (rows_j / 2 + bj / 2 - 1) / (bj / 2) : (rows_j + bj - 1) / bj);
 }
 // What a launch takes, in microseconds, from timings of 16 to 4096 tiles at contractions of 256 to 2048 on 256 CUs: a workgroup's 64 of the contraction
 // take `lat` alone on its CU and `thr` of the CU's time among others, `occ` of them share a CU, a launch costs `fix`, a further round of
-// workgroups `again`.  16-bit, per 64: 64 x 64 tiles 0.25-0.28 alone, 1.30 with 8 a CU; 128 x 128 0.40-0.8 alone, 3.1 with 8 a CU; 256 x 256 1.1-1.8,
-// 6.1 with 4 a CU.  fp32: 128 x 64 1.7-2.2, 12.6 with 8 a CU; 256 x 128 3.4-4.4, 18.8 with 4 a CU.  Adding the parts of a split contraction: a
-// launch of 2 and its bytes at 4.5 TB/s.
+// workgroups `again`.  16-bit, per 64: 64 x 64 tiles 0.27 alone, 0.42 with two a CU; 128 x 128 with four stages 0.47-0.52; with two stages 0.40-0.8
+// alone with operands in a cache, 0.87 from memory, 3.1 with 8 a CU; 256 x 256 1.1-1.8, 6.1 with 4 a CU.  fp32: 128 x 64 1.7-2.2, 12.6 with 8 a CU;
+// 256 x 128 3.4-4.4, 18.8 with 4 a CU.  Adding the parts of a split contraction: a launch of 2 and its bytes at 4.5 TB/s.
 struct LinCost { int bi, bj, occ; double thr, lat, fix, again; };
 inline const LinCost& lin_cost(int dtype, int tile) {
-  static const LinCost t[2][3] = {{{64, 64, 5, 0.165, 0.27, 4.0, 1.0}, {128, 128, 2, 0.45, 0.55, 5.0, 2.0}, {256, 256, 1, 1.55, 1.55, 8.0, 4.0}},
-                                  {{0, 0, 0, 0, 0, 0, 0}, {128, 64, 2, 1.6, 1.9, 4.0, 1.5}, {256, 128, 1, 4.5, 4.5, 9.0, 4.0}}};
+  static const LinCost t[2][4] = {{{64, 64, 2, 0.21, 0.27, 4.0, 1.0}, {128, 128, 1, 0.49, 0.49, 6.0, 4.0}, {128, 128, 2, 0.45, 0.8, 5.0, 2.0},
+                                   {256, 256, 1, 1.55, 1.55, 8.0, 4.0}},
+                                  {{0, 0, 0, 0, 0, 0, 0}, {0, 0, 0, 0, 0, 0, 0}, {128, 64, 2, 1.6, 1.9, 4.0, 1.5}, {256, 128, 1, 4.5, 4.5, 9.0, 4.0}}};
   return t[dtype == kLinF32 ? 1 : 0][tile];
 }
 inline double lin_steps_time(const LinCost& c, long groups, long steps) {
@@ -78,6 +83,7 @@ inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated
     }
   }
   lin_set_plan(pl, dtype, tile, rows_i, rows_j, kk, gated, split);
+  pl.time = best;
   return pl;
 }
 // The two products of a backward pass in one launch: the longest workgroup and the work per CU bound the time; the product with the longest
@@ -148,16 +154,33 @@ struct LinPadder {
 };
 
 // ---- forward
-constexpr long kLinFewRows = 64;       // up to here the weight's bytes are the bound: lin_rows_kernel
-struct LinForwardLayout { LinPlan plan; size_t x, w, part, total; };
+constexpr long kLinFewRows = 64;       // the largest number that lin_rows_kernel takes
+// Few rows: up to 16 the weight's bytes are the bound and lin_rows_kernel it is.  Beyond, its workgroups of 16 weight rows read all of x each, 55 KB per us
+// and CU (64 x 8192 -> 1024 in bf16 21.6 us, 64 x 4096 -> 8192 27.5), which tiles of 64 rows do not (12.7, 20.6); but those pay for joining their parts and
+// for copies of odd widths (64 x 2048 -> 2048 9.2 against 9.7, 64 x 1003 -> 1337 7.6 against 12.7).
+inline double lin_rows_time(long rows, int k, int n2, int dtype, bool gated) {
+  const long of = 128 / lin_size(dtype), blocks = (k + of - 1) / of, groups = (n2 / (gated ? 2 : 1) + 15) / 16;
+  const long staged = 8 * ((gated ? 32 : 16) + (rows <= 32 ? 32 : 64)) * 128;                // bytes of a round of a workgroup's 8 waves
+  return 3.5 + (double)((blocks + 7) / 8) * ((groups + num_cus() - 1) / num_cus()) * staged / 55e3;
+}
+struct LinForwardLayout { LinPlan plan; size_t x, w, part, total; bool few; };
 inline LinForwardLayout lin_forward_layout(long rows, int k, int n2, int dtype, bool gated) {
   LinForwardLayout l = {};
-  if (rows <= kLinFewRows) return l;
+  l.few = rows <= 16;
+  if (l.few) return l;
   l.plan = lin_plan(dtype, rows, n2, k, gated, dtype == kLinF32 ? kTileNormal : kTileSmall);
   l.x = 0;
   l.w = l.x + lin_pad_bytes(dtype, rows, k);
   l.part = l.w + lin_pad_bytes(dtype, n2, k);
   l.total = l.part + l.plan.part_bytes;
+  if (rows <= kLinFewRows) {
+    const double weight = 2.0 + (double)n2 * k * lin_size(dtype) / 4.7e6, join = lin_join_time(lin_join_bytes(rows, n2, l.plan.splits));
+    const double tiles = (l.plan.time - join > weight ? l.plan.time - join : weight) + join + (l.part ? 3.0 + 2.0 * l.part / 4.5e6 : 0.0);
+    if (tiles > 0.9 * lin_rows_time(rows, k, n2, dtype, gated)) {
+      l = {};
+      l.few = true;
+    }
+  }
   return l;
 }
 template <class T, bool GATED, class Launcher>
@@ -167,7 +190,7 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   const int n2 = GATED ? 2 * n : n;
   p.a = x; p.b = w; p.rows_i = rows; p.rows_j = n2; p.kk = k; p.lda = p.ldb = k; p.splits = 1;
   p.bias = bias; p.res = res; p.out = out; p.pre = pre; p.act = act; p.f = GATED ? n : 0;
-  if (rows <= kLinFewRows) {
+  if (l.few) {
     const int grid = (n + 15) / 16;
     if (rows <= 16) return L.launch(lin_rows_kernel<T, 1, 16, GATED>, grid, 1024, p);
     if (rows <= 32) return L.launch(lin_rows_kernel<T, 2, 8, GATED>, grid, 512, p);
@@ -186,6 +209,7 @@ int lin_forward_t(Launcher& L, int dtype, const void* x, const void* w, const vo
   if constexpr (sizeof(T) == 2) {
     if (l.plan.tile == kTileWide) rc = L.launch(lin_dma_kernel<LinD256, T, GATED>, (int)grid, LinD256::NT, p);
     else if (l.plan.tile == kTileSmall) rc = L.launch(lin_dma_kernel<LinD64, T, GATED>, (int)grid, LinD64::NT, p);
+    else if (l.plan.tile == kTileDeep) rc = L.launch(lin_dma_kernel<LinD128x4, T, GATED>, (int)grid, LinD128x4::NT, p);
     else rc = L.launch(lin_dma_kernel<LinD128, T, GATED>, (int)grid, LinD128::NT, p);
   } else {
     if (l.plan.tile == kTileWide) rc = L.launch(lin_split_kernel<LinF256, GATED>, (int)grid, LinF256::NT, p);
