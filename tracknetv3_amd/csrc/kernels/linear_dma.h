@@ -1,6 +1,7 @@
 // linear_dma.h -- the wide products of 16-bit operands: tiles move from memory to LDS by direct loads, nothing passes through registers on the way.
 //
-// A workgroup of WM x WN waves computes (TM 32 WM) x (TN 32 WN) outputs, 64 of the contraction per step, two LDS stages.  A wave owns 2 TM x 2 TN MFMA tiles (16x16x32).
+// A workgroup of WM x WN waves computes (TM 32 WM) x (TN 32 WN) outputs, 64 of the contraction per step, two LDS stages (NS in general: NS - 1
+// steps of loads are in flight, counted waits).  A wave owns 2 TM x 2 TN MFMA tiles (16x16x32).
 // One barrier per step, placed before the LAST quarter of a step's products: at that point every wave has the step's last fragments in
 // registers and its share of the next stage has landed, so behind the barrier the stage just read can be refilled (a whole step for the loads to
 // arrive) and the next step's first fragments are read under the last quarter's products.  No product waits for a read that was not issued a

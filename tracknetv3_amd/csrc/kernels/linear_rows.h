@@ -1,4 +1,5 @@
-// linear_rows.h -- forward products of few rows (single positions of a stream, small batches): bound by reading the weight once.
+// linear_rows.h -- forward products of few rows (single positions of a stream, small batches): bound by reading the weight once, beyond about 32 rows by
+// reading x once per 16 weight rows.
 //
 // A workgroup takes 16 weight rows (gated: 16 of the gate and the same 16 of the other factor) against all rows of x; its NW waves share the
 // contraction, one block of 128 bytes per row each in turn, and join their sums through LDS in a fixed order.  A block goes through registers and a
