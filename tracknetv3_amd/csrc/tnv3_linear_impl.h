@@ -11,10 +11,10 @@ namespace tnv3 {
 
 using LinD256 = LinDmaCfg<2, 4, 4, 2>;          // 256 x 256, eight waves of 64 x 128: one workgroup per CU
 using LinD128 = LinDmaCfg<2, 2, 2, 2>;          // 128 x 128, four waves of 64 x 64: two workgroups per CU
-// forward products of few tiles, whose operands come from memory rather than a cache: four LDS stages, so that three steps' loads are in flight (two
-// stages: 200 x 4096 -> 8192 in bf16 51 us instead of 31, 200 x 4096 -> 4096 32 instead of 22)
+// products of few tiles, whose operands come from memory rather than a cache: four LDS stages, so that three steps' loads are in flight (two stages:
+// 200 x 4096 -> 8192 in bf16 51 us instead of 29, 200 x 4096 -> 4096 32 instead of 21, the gradient of 1024 x 4096 alone 55 instead of 42)
 using LinD128x4 = LinDmaCfg<2, 2, 2, 2, 4>;     // 128 x 128, one workgroup per CU
-using LinD64 = LinDmaCfg<1, 2, 2, 1, 4>;        // 64 x 64, two waves of 32 x 64, two workgroups per CU
+using LinD64 = LinDmaCfg<1, 2, 2, 1, 4>;        // 64 x 64, two waves of 32 x 64, two workgroups per CU (forward)
 using LinF256 = LinSplitCfg<2, 2, 4, 2>;        // fp32: 256 x 128, eight waves of 64 x 64, one workgroup per CU (144 KB of LDS)
 using LinF128 = LinSplitCfg<1, 2, 4, 1>;        // fp32: 128 x 64, four waves of 32 x 64, two workgroups per CU
 
@@ -86,6 +86,8 @@ inline LinPlan lin_plan(int dtype, long rows_i, long rows_j, long kk, bool gated
   pl.time = best;
   return pl;
 }
+// the smallest tile of a backward pass
+inline int lin_backward_tile(int dtype) { return dtype == kLinF32 ? kTileNormal : kTileDeep; }
 // The two products of a backward pass in one launch: the longest workgroup and the work per CU bound the time; the product with the longest
 // workgroups is split further as long as that helps.
 inline void lin_pair_plan(LinPlan& dx, LinPlan& dw, int dtype, long rows, int k, int n2) {
@@ -93,7 +95,7 @@ inline void lin_pair_plan(LinPlan& dx, LinPlan& dw, int dtype, long rows, int k,
   double best = -1;
   int tile = kTileNormal;
   int choice[2] = {0, 0};
-  for (int t = kTileNormal; t <= kTileWide; ++t) {
+  for (int t = lin_backward_tile(dtype); t <= kTileWide; ++t) {
     const LinCost& c = lin_cost(dtype, t);
     const long tiles[2] = {lin_tiles(ri[0], k, false, c.bi, c.bj), lin_tiles(ri[1], k, false, c.bi, c.bj)};
     int at[2] = {0, 0};
@@ -235,8 +237,8 @@ inline LinBackwardLayout lin_backward_layout(long rows, int k, int n, int act, i
   const int n2 = gated ? 2 * n : n;
   LinBackwardLayout l = {};
   if (dx && dw) lin_pair_plan(l.dx, l.dw, dtype, rows, k, n2);
-  else if (dx) l.dx = lin_plan(dtype, rows, k, n2, false, kTileNormal);
-  else if (dw) l.dw = lin_plan(dtype, n2, k, rows, false, kTileNormal);
+  else if (dx) l.dx = lin_plan(dtype, rows, k, n2, false, lin_backward_tile(dtype));
+  else if (dw) l.dw = lin_plan(dtype, n2, k, rows, false, lin_backward_tile(dtype));
   const long per = lin_dz_rows(rows, n);
   l.dz = 0;
   l.sums = l.dz + (gated || act != kActNone ? lin_pad((size_t)rows * lin_ld(dtype, n2) * lin_size(dtype)) : lin_pad_bytes(dtype, rows, n2));
@@ -298,6 +300,7 @@ int lin_backward_t(Launcher& L, int dtype, const void* dy, const void* x, const 
   int rc;
   if constexpr (sizeof(T) == 2) {
     if (tile == kTileWide) rc = L.launch(lin_dma_pair_kernel<LinD256, T>, (int)grid, LinD256::NT, q);
+    else if (tile == kTileDeep) rc = L.launch(lin_dma_pair_kernel<LinD128x4, T>, (int)grid, LinD128x4::NT, q);
     else rc = L.launch(lin_dma_pair_kernel<LinD128, T>, (int)grid, LinD128::NT, q);
   } else {
     if (tile == kTileWide) rc = L.launch(lin_split_pair_kernel<LinF256>, (int)grid, LinF256::NT, q);
