@@ -203,3 +203,15 @@ def check_nan_stays_in_place(rows, k, n, dtype, gated, device, seed=0):
         assert torch.isnan(got["y"][:, j % n]).all() and torch.equal(got["y"][:, cols], clean["y"][:, cols]), ("w", j)
         assert torch.isnan(got["dx"]).all() and torch.isnan(got["dw"][j % n]).all()         # (gated: act'(g) u, whichever is NaN)
         assert torch.equal(got["dw"][others], clean["dw"][others]) and torch.equal(got["db"][others], clean["db"][others]), ("w", j)
+
+
+def check_sigmoid_derivative(dtype, device):
+    """sigmoid'(z) = s(z) s(-z) falls by e per unit on BOTH sides; 1 - s would be 0 from z = 17 on.  One row, W = 0, z = the bias; bounds as in
+    check_far_gates."""
+    u, k = HALF_STEP[dtype], 8
+    b = torch.tensor([-60.0, -30.0, -17.0, -8.0, 0.0, 8.0, 12.0, 17.0, 30.0, 60.0]).to(dtype)
+    scale = 1024.0 if dtype == torch.float16 else 1.0                  # (keeps fp16's results normal a little longer)
+    x, w, dy = torch.ones(1, k, dtype=dtype), torch.zeros(len(b), k, dtype=dtype), torch.full((1, len(b)), scale, dtype=dtype)
+    got = run(*(t.to(device) for t in (x, w, b)), None, "sigmoid", False, dy.to(device))["db"].cpu().double()
+    want = scale * torch.sigmoid(b.double()) * torch.sigmoid(-b.double())              # (autograd's s (1 - s) cancels in 64 bits too: 0 at 60)
+    assert ((got - want).abs() <= (2 * u + 2.0 ** -15) * want + TINY[dtype]).all(), (got.tolist(), want.tolist())

@@ -225,3 +225,8 @@ def test_a_launch_that_counts_more_than_32_bits_of_work_items_is_refused(emu):
     assert need > rows * 80 - 1
     assert lib.tnv3_linear_forward(p(t), p(t), None, None, p(t), None, p(t), need, rows, 33, 8, 0, 1, None) != 0
     assert b"more than one launch takes" in lib.tnv3_last_error()
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+def test_sigmoid_derivative_at_large_arguments(emu, dtype):
+    lc.check_sigmoid_derivative(dtype, "cpu")

@@ -286,3 +286,8 @@ def test_operands_beyond_2_to_the_32_bytes_and_elements(gpu_device, dtype):
     for at in range(0, n, 1 << 16):
         want += dy[:, at:at + (1 << 16)].float() @ w[at:at + (1 << 16)].float()
     assert want.abs().max() <= 256 and torch.equal(dx.float(), want)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+def test_sigmoid_derivative_at_large_arguments(gpu_device, dtype):
+    lc.check_sigmoid_derivative(dtype, gpu_device)

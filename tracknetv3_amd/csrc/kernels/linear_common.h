@@ -198,7 +198,7 @@ template <bool FAST> __device__ __forceinline__ void lin_act_grad1(float z, int 
   const float zc = z < -64.0f ? -64.0f : (z > 64.0f ? 64.0f : z);
   switch (act) {
     case kActLeaky: a = z > 0.0f ? z : 0.01f * z; d = z > 0.0f ? 1.0f : 0.01f; return;
-    case kActSigmoid: { const float s = lin_sigmoid<FAST>(zc); a = s; d = s * (1.0f - s); return; }
+    case kActSigmoid: { const float s = lin_sigmoid<FAST>(zc); a = s; d = s * lin_sigmoid<FAST>(-zc); return; }      // (1 - s: 0 from z = 17 on)
     case kActRelu: a = z > 0.0f ? z : (z != z ? z : 0.0f); d = z <= 0.0f ? 0.0f : 1.0f; return;
     case kActSilu: { const float s = lin_sigmoid<FAST>(zc); a = z * s; d = s * (1.0f + zc * (1.0f - s)); return; }
     case kActGelu: { const float p = lin_phi<FAST>(zc); a = z * p; d = p + 0.39894228040143268f * zc * lin_exp<FAST>(-0.5f * zc * zc); return; }
