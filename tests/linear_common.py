@@ -215,3 +215,32 @@ def check_sigmoid_derivative(dtype, device):
     got = run(*(t.to(device) for t in (x, w, b)), None, "sigmoid", False, dy.to(device))["db"].cpu().double()
     want = scale * torch.sigmoid(b.double()) * torch.sigmoid(-b.double())              # (autograd's s (1 - s) cancels in 64 bits too: 0 at 60)
     assert ((got - want).abs() <= (2 * u + 2.0 ** -15) * want + TINY[dtype]).all(), (got.tolist(), want.tolist())
+
+
+FAR_GATES = (-30.0, -70.0, -100.0, -1e3, -6e4, -1e20, -1e30, -3e38, 30.0, 70.0, 1e3, 6e4)
+
+
+def check_far_gates(act, dtype, device):
+    """Gates far from 0 (masks, large biases): one row, W = 0, so g and u are the biases; dh = 1, x = 1.  du = dh act(g) must be what the forward pass
+    multiplies with, dg = dh u act'(g) the derivative there.  Bounds: the exponential's argument carries |g| 2^-24 and the function 2^-21, so 2^-15
+    relative at |g| <= 128; below, either side is 0 to within 128 times the least normal number; one rounding to the type for dz and one for each
+    result."""
+    u, k = HALF_STEP[dtype], 8
+    gates = torch.tensor([g for g in FAR_GATES if abs(g) <= torch.finfo(dtype).max], dtype=torch.float64).to(dtype)
+    n = len(gates)
+    b = torch.cat([gates, torch.full((n,), 1.5).to(dtype)])
+    x, w, dy = torch.ones(1, k, dtype=dtype), torch.zeros(2 * n, k, dtype=dtype), torch.ones(1, n, dtype=dtype)
+    got = {q: v.cpu().double() for q, v in run(*(t.to(device) for t in (x, w, b)), None, act, True, dy.to(device)).items()}
+    want = oracle(x, w, b, None, act, True, dy)
+    if act == "sigmoid":                                               # (autograd's s (1 - s) cancels in 64 bits too)
+        dg = 1.5 * torch.sigmoid(gates.double()) * torch.sigmoid(-gates.double())
+        want["db"][:n], want["dw"][:n] = dg, dg[:, None].expand(n, k)
+    floor = 2 * max(TINY[dtype], 128 * 2.0 ** -126)
+    for name, rel in (("y", u + 2.0 ** -15), ("db", 2 * u + 2.0 ** -15), ("dw", 2 * u + 2.0 ** -15)):
+        fits = want[name].abs() <= torch.finfo(dtype).max              # 1.5 * 6e4 is beyond fp16's largest: infinite
+        assert torch.equal(torch.isfinite(got[name]), fits), name
+        err = (got[name] - want[name]).abs()
+        assert (err <= rel * want[name].abs() + floor)[fits].all(), (name, got[name].tolist(), want[name].tolist())
+    # the same activation in both directions: y = 1.5 act(g), db's second half act(g)
+    fits = torch.isfinite(got["y"][0])
+    assert ((got["y"][0] - 1.5 * got["db"][n:]).abs() <= 4 * u * got["y"][0].abs() + 2 * floor)[fits].all()

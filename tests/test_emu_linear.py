@@ -230,3 +230,9 @@ def test_a_launch_that_counts_more_than_32_bits_of_work_items_is_refused(emu):
 @pytest.mark.parametrize("dtype", lc.DTYPES)
 def test_sigmoid_derivative_at_large_arguments(emu, dtype):
     lc.check_sigmoid_derivative(dtype, "cpu")
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("act", [a for a in lc.ACTS if a != "none"])
+def test_gates_far_from_zero(emu, act, dtype):
+    lc.check_far_gates(act, dtype, "cpu")

@@ -291,3 +291,9 @@ def test_operands_beyond_2_to_the_32_bytes_and_elements(gpu_device, dtype):
 @pytest.mark.parametrize("dtype", lc.DTYPES)
 def test_sigmoid_derivative_at_large_arguments(gpu_device, dtype):
     lc.check_sigmoid_derivative(dtype, gpu_device)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("act", [a for a in lc.ACTS if a != "none"])
+def test_gates_far_from_zero(gpu_device, act, dtype):
+    lc.check_far_gates(act, dtype, gpu_device)

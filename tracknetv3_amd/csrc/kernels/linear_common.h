@@ -192,10 +192,11 @@ template <bool FAST> __device__ __forceinline__ float lin_act1(float z, int act)
     default: return z;
   }
 }
-// (act(z), act'(z)); arguments are clamped to +-64 inside the derivative (NaN kept): beyond it the derivative is 0 or 1 in fp32, and products
-// like z * (1 - sigmoid(z)) would be inf * 0
+// (act(z), act'(z)), act(z) the forward pass's own value.  Inside the exponentials and the derivative, arguments are clamped to +-128 (NaN kept): there
+// sigmoid and Phi are exactly 0 or 1 in fp32 (e^-128 is below its least subnormal 2^-149 = e^-103.3), so nothing changes beyond, and products like
+// z * (1 - sigmoid(z)) never are inf * 0.  (A clamp inside that range would show: z sigmoid(-64) is -160 at z = -1e30.)
 template <bool FAST> __device__ __forceinline__ void lin_act_grad1(float z, int act, float& a, float& d) {
-  const float zc = z < -64.0f ? -64.0f : (z > 64.0f ? 64.0f : z);
+  const float zc = z < -128.0f ? -128.0f : (z > 128.0f ? 128.0f : z);
   switch (act) {
     case kActLeaky: a = z > 0.0f ? z : 0.01f * z; d = z > 0.0f ? 1.0f : 0.01f; return;
     case kActSigmoid: { const float s = lin_sigmoid<FAST>(zc); a = s; d = s * lin_sigmoid<FAST>(-zc); return; }      // (1 - s: 0 from z = 17 on)
