@@ -244,3 +244,25 @@ def check_far_gates(act, dtype, device):
     # the same activation in both directions: y = 1.5 act(g), db's second half act(g)
     fits = torch.isfinite(got["y"][0])
     assert ((got["y"][0] - 1.5 * got["db"][n:]).abs() <= 4 * u * got["y"][0].abs() + 2 * floor)[fits].all()
+
+
+def check_gelu_tail(act, dtype, device):
+    """GELU and its derivative for z in [-10, -3], RELATIVE: y is a product z Phi(z), and Phi is known to its own rounding there.  One row, W = 0, z = the
+    bias.  The exponent (up to 87 in the tanh form, after four roundings) carries 87 * 4 * 2^-24, the fitted factor 2^-17: 2^-14 together, and Phi + z phi
+    amplifies it by at most (z^2 + 1) / (z^2 - 1) <= 1.25."""
+    u, k = HALF_STEP[dtype], 8
+    b = torch.linspace(-10.0, -3.0, 57).to(dtype)
+    z = b.double()
+    if act == "gelu":
+        p, dp = 0.5 * torch.special.erfc(-z / 2 ** 0.5), torch.exp(-0.5 * z * z) / (2 * torch.pi) ** 0.5
+    else:                                                              # (1 + tanh a) / 2 = sigmoid(2 a)
+        c = (2 / torch.pi) ** 0.5
+        a = 2 * c * (z + 0.044715 * z ** 3)
+        p = torch.sigmoid(a)
+        dp = p * torch.sigmoid(-a) * 2 * c * (1 + 3 * 0.044715 * z * z)
+    want = {"y": (z * p)[None], "db": p + z * dp}
+    x, w, dy = torch.ones(1, k, dtype=dtype), torch.zeros(len(b), k, dtype=dtype), torch.ones(1, len(b), dtype=dtype)
+    got = run(*(t.to(device) for t in (x, w, b)), None, act, False, dy.to(device))
+    for name, rel in (("y", u + 2.0 ** -14), ("db", 2 * u + 2.0 ** -13)):
+        err = (got[name].cpu().double() - want[name]).abs()
+        assert (err <= rel * want[name].abs() + TINY[dtype]).all(), (name, (err / want[name].abs()).tolist())

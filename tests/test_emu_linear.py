@@ -236,3 +236,9 @@ def test_sigmoid_derivative_at_large_arguments(emu, dtype):
 @pytest.mark.parametrize("act", [a for a in lc.ACTS if a != "none"])
 def test_gates_far_from_zero(emu, act, dtype):
     lc.check_far_gates(act, dtype, "cpu")
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
+def test_gelu_of_negative_arguments_to_relative_accuracy(emu, act, dtype):
+    lc.check_gelu_tail(act, dtype, "cpu")

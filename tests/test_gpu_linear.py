@@ -297,3 +297,9 @@ def test_sigmoid_derivative_at_large_arguments(gpu_device, dtype):
 @pytest.mark.parametrize("act", [a for a in lc.ACTS if a != "none"])
 def test_gates_far_from_zero(gpu_device, act, dtype):
     lc.check_far_gates(act, dtype, gpu_device)
+
+
+@pytest.mark.parametrize("dtype", lc.DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
+def test_gelu_of_negative_arguments_to_relative_accuracy(gpu_device, act, dtype):
+    lc.check_gelu_tail(act, dtype, gpu_device)
