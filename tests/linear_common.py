@@ -266,3 +266,14 @@ def check_gelu_tail(act, dtype, device):
     for name, rel in (("y", u + 2.0 ** -14), ("db", 2 * u + 2.0 ** -13)):
         err = (got[name].cpu().double() - want[name]).abs()
         assert (err <= rel * want[name].abs() + TINY[dtype]).all(), (name, (err / want[name].abs()).tolist())
+
+
+def check_least_positive(rows, k, n, act, device):
+    """fp16: a positive pre-activation below the type's least subnormal has the derivative 1, not that of 0.  z = 2^-14 * 2^-13 in every element (exact),
+    so y rounds to 0 while dz = dy."""
+    x, w = torch.zeros(rows, k, dtype=torch.float16), torch.zeros(n, k, dtype=torch.float16)
+    x[:, -1], w[:, -1] = 2.0 ** -14, 2.0 ** -13
+    dy = torch.ones(rows, n, dtype=torch.float16)
+    got = run(x.to(device), w.to(device), torch.zeros(n, dtype=torch.float16, device=device), None, act, False, dy.to(device))
+    assert not got["y"].any()
+    assert (got["db"].cpu() == rows).all() and (got["dx"][:, -1].cpu().double() == n * 2.0 ** -13).all()

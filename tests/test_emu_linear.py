@@ -242,3 +242,9 @@ def test_gates_far_from_zero(emu, act, dtype):
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
 def test_gelu_of_negative_arguments_to_relative_accuracy(emu, act, dtype):
     lc.check_gelu_tail(act, dtype, "cpu")
+
+
+@pytest.mark.parametrize("act", ["relu", "leaky_relu"])
+@pytest.mark.parametrize("rows,k,n", [(2, 24, 16), (3, 9, 11), (70, 72, 24), (70, 1096, 20)])         # few rows; odd; tiles; tiles with parts to join
+def test_least_positive_pre_activation(emu, rows, k, n, act):
+    lc.check_least_positive(rows, k, n, act, "cpu")

@@ -303,3 +303,9 @@ def test_gates_far_from_zero(gpu_device, act, dtype):
 @pytest.mark.parametrize("act", ["gelu", "gelu_tanh"])
 def test_gelu_of_negative_arguments_to_relative_accuracy(gpu_device, act, dtype):
     lc.check_gelu_tail(act, dtype, gpu_device)
+
+
+@pytest.mark.parametrize("act", ["relu", "leaky_relu"])
+@pytest.mark.parametrize("rows,k,n", [(2, 24, 16), (3, 9, 11), (70, 72, 24), (70, 1096, 20), (1500, 520, 1032)])
+def test_least_positive_pre_activation(gpu_device, rows, k, n, act):
+    lc.check_least_positive(rows, k, n, act, gpu_device)

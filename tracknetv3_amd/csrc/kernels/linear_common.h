@@ -103,6 +103,11 @@ __device__ __forceinline__ void lin_down(float f, float& o) { o = f; }
 // the fp32 value that an element of type T keeps of f
 template <class T> __device__ __forceinline__ float lin_round(float f) { T t; lin_down(f, t); return lin_up(t); }
 
+// A pre-activation as a backward pass takes it: rounded to T, but no positive value to 0 -- in fp16 those below 2^-25 would be, and ReLU's derivative at 0
+// is another one.
+template <class T> __device__ __forceinline__ float lin_keep_positive(float z) { return z; }
+template <> __device__ __forceinline__ float lin_keep_positive<LinF16>(float z) { return z > 0.0f && z < 0x1p-24f ? 0x1p-24f : z; }
+
 // ---- eight consecutive elements <-> fp32.  vec: all eight exist; else the first `n` one by one (the rest 0).
 __device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinBf16) {
 #pragma unroll
@@ -158,6 +163,13 @@ template <> __device__ __forceinline__ void lin_store8<float>(float* p, const fl
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < n) p[i] = v[i];
+}
+
+template <class T> __device__ __forceinline__ void lin_store_pre8(T* p, const float (&v)[8], bool vec, int n) {
+  float z[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) z[i] = lin_keep_positive<T>(v[i]);
+  lin_store8<T>(p, z, vec, n);
 }
 
 // ---- activations.  FAST (16-bit outputs): hardware exp2 and reciprocal, each within about 2^-23; the exponential's argument x carries |x| 2^-24 besides,
@@ -321,7 +333,7 @@ __device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j
   const long o = i * p.rows_j + j;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
-  if (p.pre) lin_store8<T>(static_cast<T*>(p.pre) + o, v, vec, n);
+  if (p.pre) lin_store_pre8<T>(static_cast<T*>(p.pre) + o, v, vec, n);
   lin_act8<sizeof(T) == 2>(v, p.act);
   if (p.res) {
     float r[8];
@@ -462,7 +474,7 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, flo
                 lin_store8<float>(static_cast<float*>(p.pre) + o, v[q], true, 8);
                 lin_store8<float>(static_cast<float*>(p.pre) + o + p.f, u[GATED ? q : 0], true, 8);
               } else {
-                lin_store8<T>(static_cast<T*>(p.pre) + o, v[q], true, 8);
+                lin_store_pre8<T>(static_cast<T*>(p.pre) + o, v[q], true, 8);
               }
             }
         }

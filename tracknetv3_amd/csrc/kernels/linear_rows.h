@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(NW * 64) lin_rows_kernel(const LinGemmArgs p) 
       lin_down(lin_act1<FAST>(v, p.act) * u, static_cast<T*>(p.out)[i * p.f + j]);
     } else {
       const long o = i * p.rows_j + j;
-      if (p.pre) lin_down(v, static_cast<T*>(p.pre)[o]);
+      if (p.pre) lin_down(lin_keep_positive<T>(v), static_cast<T*>(p.pre)[o]);
       v = lin_act1<FAST>(v, p.act);
       if (p.res) v += lin_up(static_cast<const T*>(p.res)[o]);
       lin_down(v, static_cast<T*>(p.out)[o]);
