@@ -68,3 +68,16 @@ extern "C" long tnv3_emu_tile_walk_check(void) {
         }
   return checked;
 }
+
+// What a position-wise product is launched as.  which: 0 the forward product, 1 / 2 the gradient of x / of the weight where both are wanted, 3 / 4 where
+// one alone is.  -1: the few-rows kernel; else tile (LinPlan::tile) + 256 * the contraction's parts.
+extern "C" int tnv3_emu_linear_plan(int which, long rows, int k, int n, int dtype, int gated) {
+  init_cu_count();
+  if (which == 0) {
+    const tnv3::LinForwardLayout l = tnv3::lin_forward_layout(rows, k, gated ? 2 * n : n, dtype, gated != 0);
+    return l.few ? -1 : l.plan.tile + 256 * l.plan.splits;
+  }
+  const tnv3::LinBackwardLayout l = tnv3::lin_backward_layout(rows, k, n, 1, dtype, gated != 0, which != 4, which != 3);
+  const tnv3::LinPlan& p = which == 1 || which == 3 ? l.dx : l.dw;
+  return p.tile + 256 * p.splits;
+}

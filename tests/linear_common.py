@@ -277,3 +277,110 @@ def check_least_positive(rows, k, n, act, device):
     got = run(x.to(device), w.to(device), torch.zeros(n, dtype=torch.float16, device=device), None, act, False, dy.to(device))
     assert not got["y"].any()
     assert (got["db"].cpu() == rows).all() and (got["dx"][:, -1].cpu().double() == n * 2.0 ** -13).all()
+
+
+# Every product kernel by sizes that are planned on it: (16-bit types?, gated, which: 0 forward, 1 both gradients, tile: 0 64 x 64, 1 128 x 128 with four LDS
+# stages, 2 128 x 128 / fp32 128 x 64, 3 256 x 256 / fp32 256 x 128, contraction in parts?, sizes).  For the emulator's CU count (first column) and the card's 256.
+KERNELS_EMU = [
+    (1, True, False, 0, 0, False, (65, 40, 40)), (1, True, False, 0, 1, False, (65, 200, 72)), (1, True, False, 0, 2, False, (65, 40, 72)),
+    (4, True, False, 0, 3, False, (257, 392, 392)), (2, True, True, 0, 0, False, (65, 40, 40)), (1, True, True, 0, 1, False, (65, 200, 40)),
+    (1, True, True, 0, 2, False, (65, 40, 40)), (1, True, True, 0, 3, False, (130, 264, 72)),
+    (4, True, False, 1, 1, False, (257, 40, 40)), (4, True, False, 1, 2, True, (200, 40, 40)), (4, True, False, 1, 3, False, (130, 264, 136)),
+    (4, True, False, 1, 3, True, (130, 136, 392)), (4, True, True, 1, 1, False, (65, 40, 136)), (2, True, True, 1, 2, True, (65, 40, 520)),
+    (4, True, True, 1, 3, True, (130, 136, 200)),
+    (1, False, False, 0, 2, False, (65, 40, 40)), (2, False, False, 0, 2, True, (65, 136, 40)), (1, False, False, 0, 3, False, (130, 72, 72)),
+    (4, False, True, 0, 2, True, (65, 136, 40)), (1, False, True, 0, 3, False, (130, 72, 40)),
+    (4, False, False, 1, 2, True, (130, 40, 40)), (1, False, False, 1, 3, False, (130, 72, 136)), (1, False, False, 1, 3, True, (130, 72, 520)),
+    (1, False, True, 1, 2, True, (65, 40, 200)), (4, False, True, 1, 3, True, (130, 72, 136)),
+]
+KERNELS_GPU = [(256,) + e for e in (
+    (True, False, 0, 0, True, (65, 776, 72)), (True, False, 0, 1, False, (1500, 200, 2056)), (True, False, 0, 1, True, (65, 4104, 4104)),
+    (True, False, 0, 2, False, (1500, 40, 2056)), (True, False, 0, 2, True, (2500, 4104, 776)), (True, False, 0, 3, False, (3001, 264, 4104)),
+    (True, True, 0, 0, True, (65, 776, 72)), (True, True, 0, 1, False, (260, 200, 5000)), (True, True, 0, 1, True, (65, 2056, 4104)),
+    (True, True, 0, 2, False, (260, 40, 5000)), (True, True, 0, 2, True, (200, 4104, 4104)), (True, True, 0, 3, False, (4100, 72, 5000)),
+    (True, False, 1, 1, True, (200, 40, 4104)), (True, False, 1, 2, True, (200, 40, 72)), (True, False, 1, 3, False, (1500, 4104, 1544)),
+    (True, False, 1, 3, True, (4100, 1544, 520)), (True, True, 1, 1, True, (65, 40, 4104)), (True, True, 1, 2, True, (200, 40, 72)),
+    (True, True, 1, 3, False, (1500, 4104, 776)), (True, True, 1, 3, True, (65, 4104, 4104)),
+    (False, False, 0, 2, True, (65, 136, 72)), (False, False, 0, 3, False, (1500, 72, 4104)), (False, False, 0, 3, True, (130, 2056, 4104)),
+    (False, True, 0, 2, True, (65, 136, 72)), (False, True, 0, 3, False, (520, 72, 5000)), (False, True, 0, 3, True, (130, 520, 4104)),
+    (False, False, 1, 2, True, (65, 40, 136)), (False, False, 1, 3, False, (520, 4104, 520)), (False, False, 1, 3, True, (130, 520, 4104)),
+    (False, True, 1, 2, True, (65, 40, 72)), (False, True, 1, 3, False, (520, 4104, 264)), (False, True, 1, 3, True, (130, 520, 2056)))]
+
+
+def check_kernel(half, gated, rows, k, n, device):
+    """One kernel of KERNELS_*: bias, activation, residual and a kept pre-activation in the epilogue; real values against the bounds, integers exactly, and in
+    fp32 integers that fill all three planes."""
+    for dtype in ((torch.bfloat16, torch.float16) if half else (torch.float32,)):
+        check_close(rows, k, n, dtype, "silu", gated, bias=True, residual=not gated, device=device, seed=rows + k + n)
+        check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device=device, seed=rows + n)
+        if dtype == torch.float32:
+            check_exact_planes(rows, k, n, gated, device)
+
+
+def check_exact_planes(rows, k, n, gated, device):
+    """fp32 products of integers of up to 24 bits: three planes on one side, or two on both, so that every one of the six plane products carries part of the
+    result.  All sums of absolute values stay within 2^24: exact in any order, so the results are equal."""
+    gen = torch.Generator().manual_seed(rows + k + n)
+
+    def integers(shape, bits, density):
+        v = torch.randint(1, 1 << bits, shape, generator=gen) * (torch.randint(0, 2, shape, generator=gen) * 2 - 1) if bits else \
+            torch.randint(0, 2, shape, generator=gen) * 2 - 1
+        return (v * (torch.rand(shape, generator=gen) < density)).double()
+    for bits_x, bits_w in ((20, 0), (0, 20), (10, 10)):
+        # x, w and dy meet pairwise over k, n and rows; about 1.5 products per sum, of up to 2^20
+        p = (1.5 / max(k, n, rows)) ** 0.5
+        x, w, dy = integers((rows, k), bits_x, p), integers((n, k), bits_w, p), integers((rows, n), 0, p)
+        if gated:                             # u = 1 by a column of its own: h = g
+            x[:, 0], w[:, 0] = 1, 0
+            up = torch.zeros(n, k, dtype=torch.float64)
+            up[:, 0] = 1
+            got = ops_call("gated_linear", x, torch.cat([w, up]), device)
+            assert (x.abs() @ w.abs().t()).max() <= 1 << 24
+            assert torch.equal(got, x @ w.t()), (bits_x, bits_w)
+            continue
+        sums = [(x, w.t()), (dy, w), (dy.t(), x)]
+        assert all((a.abs() @ b.abs()).max() <= 1 << 24 for a, b in sums)
+        y = ops_call("linear", x, w, device)
+        dx, dw, _ = ops_call("linear_backward", dy, x, w, device)
+        for name, got, (a, b) in zip(("y", "dx", "dw"), (y, dx, dw), sums):
+            assert torch.equal(got, a @ b), (name, bits_x, bits_w, (got != a @ b).nonzero()[:4].tolist())
+
+
+def ops_call(name, *args):
+    """ops.<name> of float64 tensors in fp32 on the device that comes last, without an activation; float64 results."""
+    from tracknetv3_amd import ops
+    out = getattr(ops, name)(*(t.float().to(args[-1]) for t in args[:-1]), act=ops.ACT_NONE)
+    return tuple(t if t is None else t.cpu().double() for t in out) if isinstance(out, tuple) else out.cpu().double()
+
+
+def check_nonfinite_products(rows, k, n, device, seed=0):
+    """fp32, all three products (y = x w^T, dx = dy w, dw = dy^T x), with infinities of either sign, NaN and values beyond bf16's largest in either operand:
+    NaN, infinities and their signs where fp32 arithmetic has them, the finite rest to its usual accuracy."""
+    from tracknetv3_amd import ops
+    inf, nan, big = float("inf"), float("nan"), 3.4e38
+    for where in ("x", "w", "dy"):
+        gen = torch.Generator().manual_seed(seed + rows + n)
+        t = {"x": torch.randn(rows, k, generator=gen), "w": torch.randn(n, k, generator=gen), "dy": torch.randn(rows, n, generator=gen)}
+        # beyond bf16's largest: only products with factors of at most 1/8 in size, so that no sum of them passes fp32's largest
+        for q in t:
+            t[q] = t[q].clamp(-4, 4) if q == where else t[q].clamp(-4, 4) / 64
+        a, b = t[where].shape
+        for at, v in (((1, 3), inf), ((2, 7), -inf), ((3, 2), nan), ((4, 0), big), ((a - 1, b - 1), -inf), ((a // 2, b // 2), -big)):
+            t[where][at] = v
+        for q in t:                            # inf * 0 = NaN
+            if q != where:
+                t[q][5, 3] = t[q][3, 5] = 0.0
+        x, w, dy = (t[q].to(device) for q in ("x", "w", "dy"))
+        y = ops.linear(x, w)
+        dx, dw, _ = ops.linear_backward(dy, x, w)
+        for name, got, (p, q) in (("y", y, ("x", "wt")), ("dx", dx, ("dy", "w")), ("dw", dw, ("dyt", "x"))):
+            p, q = ((t[s[:-1]].t() if s.endswith("t") else t[s]).double() for s in (p, q))
+            want, got = (p @ q).float(), got.cpu()
+            assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isinf(got), torch.isinf(want)), (where, name)
+            at = torch.isinf(want)
+            assert torch.equal(torch.sign(got[at]), torch.sign(want[at])), (where, name)
+            ok = torch.isfinite(want)
+            # a finite sum: the chain's roundings and the split's 2^-23 per term, relative to the sum of the sizes
+            size = torch.where(torch.isfinite(p), p, 0.0).abs() @ torch.where(torch.isfinite(q), q, 0.0).abs()
+            limit = ((6 * p.shape[1] / 16 + 64) * 2.0 ** -24 + 2.0 ** -23) * size + 2.0 ** -126
+            assert ((got.double() - p @ q).abs()[ok] <= limit[ok]).all(), (where, name)

@@ -248,3 +248,44 @@ def test_gelu_of_negative_arguments_to_relative_accuracy(emu, act, dtype):
 @pytest.mark.parametrize("rows,k,n", [(2, 24, 16), (3, 9, 11), (70, 72, 24), (70, 1096, 20)])         # few rows; odd; tiles; tiles with parts to join
 def test_least_positive_pre_activation(emu, rows, k, n, act):
     lc.check_least_positive(rows, k, n, act, "cpu")
+
+
+def _plan(emu, which, rows, k, n, half, gated):
+    """(tile, parts of the contraction: the most of both products') of a launch; the few-rows kernel has tile -1."""
+    call = emu.load().tnv3_emu_linear_plan
+    call.argtypes = [ctypes.c_int, ctypes.c_long] + [ctypes.c_int] * 4
+    got = [call(q, rows, k, n, int(half), int(gated)) for q in ((0,) if which == 0 else (1, 2))]
+    return (-1, 1) if got[0] < 0 else (got[0] % 256, max(g // 256 for g in got))
+
+
+@pytest.mark.parametrize("cus,half,gated,which,tile,parts,sizes", lc.KERNELS_EMU + lc.KERNELS_GPU)
+def test_sizes_are_planned_on_the_kernel_they_are_to_test(emu, monkeypatch, cus, half, gated, which, tile, parts, sizes):
+    monkeypatch.setenv("TNV3_EMU_CUS", str(cus))
+    got = _plan(emu, which, *sizes, half, gated)
+    assert (got[0], got[1] > 1) == (tile, parts)
+
+
+def test_every_kernel_is_listed():
+    want = {(half, gated, which, tile) for half in (True, False) for gated in (False, True) for which in (0, 1) for tile in range(4)
+            if (tile >= 2 or half) and (tile or which == 0)}
+    for table in (lc.KERNELS_EMU, lc.KERNELS_GPU):
+        assert {e[1:5] for e in table} == want
+
+
+@pytest.mark.parametrize("lazy", ["0", "1"])
+@pytest.mark.parametrize("cus,half,gated,which,tile,parts,sizes", lc.KERNELS_EMU)
+def test_every_kernel_by_the_sizes_that_choose_it(emu, monkeypatch, cus, half, gated, which, tile, parts, sizes, lazy):
+    """(lazy: direct loads land as early or as late as the program's waits allow)"""
+    if lazy == "1" and not half:
+        pytest.skip("fp32 products have no direct loads")
+    monkeypatch.setenv("TNV3_EMU_CUS", str(cus))
+    monkeypatch.setenv("TNV3_EMU_LAZY_DMA", lazy)
+    lc.check_kernel(half, gated, *sizes, "cpu")
+
+
+@pytest.mark.parametrize("cus,tiles,sizes", [(1, (2, 2), (70, 40, 40)), (1, (3, 2), (130, 72, 72)), (1, (2, 3), (130, 72, 136)), (4, (2, 2), (65, 136, 40))])
+def test_fp32_tiles_keep_infinities_and_nan_where_they_belong(emu, monkeypatch, cus, tiles, sizes):
+    """The products that are computed a second time, forward and backward, in both tiles, whole and in parts."""
+    monkeypatch.setenv("TNV3_EMU_CUS", str(cus))
+    assert tuple(_plan(emu, which, *sizes, False, False)[0] for which in (0, 1)) == tiles
+    lc.check_nonfinite_products(*sizes, "cpu")

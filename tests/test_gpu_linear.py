@@ -309,3 +309,17 @@ def test_gelu_of_negative_arguments_to_relative_accuracy(gpu_device, act, dtype)
 @pytest.mark.parametrize("rows,k,n", [(2, 24, 16), (3, 9, 11), (70, 72, 24), (70, 1096, 20), (1500, 520, 1032)])
 def test_least_positive_pre_activation(gpu_device, rows, k, n, act):
     lc.check_least_positive(rows, k, n, act, gpu_device)
+
+
+@pytest.mark.parametrize("cus,half,gated,which,tile,parts,sizes", lc.KERNELS_GPU)
+def test_every_kernel_by_the_sizes_that_choose_it(gpu_device, cus, half, gated, which, tile, parts, sizes):
+    """(The CPU tests check that these sizes are planned on these kernels.)"""
+    if torch.cuda.get_device_properties(gpu_device).multi_processor_count != cus:
+        pytest.skip("other CU counts plan other tiles")
+    lc.check_kernel(half, gated, *sizes, gpu_device)
+
+
+@pytest.mark.parametrize("sizes", [(70, 40, 40), (200, 40, 66), (1500, 72, 4104), (520, 4104, 520), (130, 520, 4104)])
+def test_fp32_tiles_keep_infinities_and_nan_where_they_belong(gpu_device, sizes):
+    """The products that are computed a second time, forward and backward: tiles of 128 x 64 and 256 x 128, whole and in parts."""
+    lc.check_nonfinite_products(*sizes, gpu_device)
