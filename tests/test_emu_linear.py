@@ -289,3 +289,23 @@ def test_fp32_tiles_keep_infinities_and_nan_where_they_belong(emu, monkeypatch, 
     monkeypatch.setenv("TNV3_EMU_CUS", str(cus))
     assert tuple(_plan(emu, which, *sizes, False, False)[0] for which in (0, 1)) == tiles
     lc.check_nonfinite_products(*sizes, "cpu")
+
+
+@pytest.mark.parametrize("frozen", [False, True])
+def test_a_forward_mode_tangent_is_refused(emu, frozen):
+    """Whether or not anything requires a gradient, and whichever input carries it."""
+    import torch.autograd.forward_ad as fwd
+    x, w, b, r, _ = lc.make(3, 8, 6, torch.float32, residual=True)
+    w.requires_grad_(not frozen)
+    for i in range(4):
+        with fwd.dual_level():
+            args = [x, w, b, r]
+            args[i] = fwd.make_dual(args[i].detach(), torch.ones_like(args[i]))
+            with pytest.raises(NotImplementedError):
+                ff.linear(*args)
+            if i < 3:
+                with pytest.raises(NotImplementedError):
+                    ff.gated_linear(*args[:3])
+            assert ff.linear(x, w.detach(), b, r).shape == (3, 6)                # a level is open, no input carries a tangent
+    with fwd.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
+        ff.GatedFeedForward(8, 4)(fwd.make_dual(x, torch.ones_like(x)))

@@ -16,6 +16,7 @@ import math
 
 import torch
 from torch import nn
+from torch.autograd import forward_ad
 
 from . import ops
 
@@ -29,6 +30,12 @@ def _act(act):
             raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
         return ACTIVATIONS[act]
     return act
+
+
+# There is no forward-mode derivative.  autograd says so where an input requires a gradient; otherwise the call would return an output without a tangent.
+def _no_tangents(what, *tensors):
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: an input carries a forward-mode tangent, and the position-wise layers have no forward-mode derivative")
 
 
 # (The backward passes call the ops' unchecked form: every tensor is the forward's own or has the shape and type that autograd guarantees, on the
@@ -105,7 +112,7 @@ class _GatedLinear(torch.autograd.Function):
 
 def linear(x, weight, bias=None, residual=None, act="none"):
     """act(x weight^T + bias) + residual; x (..., k), weight (n, k), bias (n,), residual (..., n), all of one type.  act: a name of ACTIVATIONS
-    or an ops.ACT_* constant.  Differentiable in every tensor."""
+    or an ops.ACT_* constant.  Differentiable once in every tensor, by a backward pass (a forward-mode tangent is refused)."""
     act = _act(act)
     x = x if x.is_contiguous() else x.contiguous()
     weight = weight if weight.is_contiguous() else weight.contiguous()
@@ -114,18 +121,20 @@ def linear(x, weight, bias=None, residual=None, act="none"):
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
+    _no_tangents("linear", x, weight, bias, residual)
     return ops.linear(x, weight, bias, residual, act)
 
 
 def gated_linear(x, weight, bias=None, act="silu"):
-    """act(g) * u with [g | u] = x weight^T + bias; x (..., k), weight (2 n, k) with the gate's n rows first, bias (2 n,).  Differentiable in every
-    tensor."""
+    """act(g) * u with [g | u] = x weight^T + bias; x (..., k), weight (2 n, k) with the gate's n rows first, bias (2 n,).  Differentiable as
+    `linear` is."""
     act = _act(act)
     x = x if x.is_contiguous() else x.contiguous()
     weight = weight if weight.is_contiguous() else weight.contiguous()
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, act)
+    _no_tangents("gated_linear", x, weight, bias)
     return ops.gated_linear(x, weight, bias, act)
 
 
