@@ -309,3 +309,18 @@ def test_a_forward_mode_tangent_is_refused(emu, frozen):
             assert ff.linear(x, w.detach(), b, r).shape == (3, 6)                # a level is open, no input carries a tangent
     with fwd.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError):
         ff.GatedFeedForward(8, 4)(fwd.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.filterwarnings("ignore")
+@pytest.mark.parametrize("frozen", [False, True])
+def test_tracing_is_refused(emu, frozen):
+    """A traced block would return uninitialised memory."""
+    block = ff.GatedFeedForward(8, 16).requires_grad_(not frozen)
+    for check in (True, False):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            torch.jit.trace(block, torch.randn(3, 8), check_trace=check)
+    x, w = torch.randn(3, 8), torch.randn(6, 8)
+    for call in (lambda t: ops.linear(t, w), lambda t: ops.gated_linear(t, w), lambda t: ops.linear_backward(t, x, torch.randn(8, 8))[0]):
+        with pytest.raises(RuntimeError, match="torch.jit.trace"):
+            torch.jit.trace(call, x, check_trace=False)
+    assert block(x).shape == (3, 8)

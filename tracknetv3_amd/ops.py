@@ -1167,6 +1167,8 @@ _LINEAR_WORKSPACE = {}          # (entry, device, sizes ..) -> bytes: a pure fun
 
 def _linear_check(what, x, weight, bias, act, gated):
     """(rows, k, n, dtype code) of a position-wise layer's call after its checks."""
+    if torch._C._get_tracing_state() is not None:          # a trace would hold the outputs' allocations and nothing that fills them
+        raise _lib.Tnv3Error(f"{what}: cannot be recorded by torch.jit.trace")
     code = _LINEAR_DTYPES.get(x.dtype)
     if code is None:
         raise _lib.Tnv3Error(f"{what}: expected float32, bfloat16 or float16, got {x.dtype}")
