@@ -324,3 +324,34 @@ def test_tracing_is_refused(emu, frozen):
         with pytest.raises(RuntimeError, match="torch.jit.trace"):
             torch.jit.trace(call, x, check_trace=False)
     assert block(x).shape == (3, 8)
+
+
+def test_streams_of_the_nodes_that_take_the_gradients():
+    """What a captured backward pass is judged by: one entry per gradient that this pass wants, read from autograd's nodes whatever operation made them.
+    (On the CPU a node has no stream, -1.)"""
+    seen = []
+
+    class Probe(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, w, b, r):
+            return x * w + r
+
+        @staticmethod
+        def backward(ctx, g):
+            seen.append(_lib.gradient_streams(ctx))
+            return g, g, None, g
+    x, w, r = torch.ones(3), torch.ones(3, requires_grad=True), torch.ones(3, requires_grad=True)
+    inner = w * 2
+    y = Probe.apply(x, inner, None, r)
+    torch.autograd.grad(y, [r], torch.ones(3), retain_graph=True)
+    torch.autograd.grad(y, [r, w], torch.ones(3), retain_graph=True)
+    y.sum().backward()
+    assert seen == [[-1], [-1, -1], [-1, -1]]
+
+
+@pytest.mark.parametrize("streams,refused", [([], False), ([-1], False), ([0], True), ([94, 0], True), ([94, 7, 94], False)])
+def test_which_captured_backward_passes_are_refused(streams, refused):
+    if not refused:
+        return ff._refuse_default_stream(streams)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        ff._refuse_default_stream(streams)

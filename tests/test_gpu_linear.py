@@ -323,3 +323,65 @@ def test_every_kernel_by_the_sizes_that_choose_it(gpu_device, cus, half, gated, 
 def test_fp32_tiles_keep_infinities_and_nan_where_they_belong(gpu_device, sizes):
     """The products that are computed a second time, forward and backward: tiles of 128 x 64 and 256 x 128, whole and in parts."""
     lc.check_nonfinite_products(*sizes, gpu_device)
+
+
+def _captured_gradients(block, x, dy, params):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(block(x), params, dy)
+    return graph, got
+
+
+def _replays_equal(graph, got, want):
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_accumulators_that_another_operation_made(gpu_device):
+    """A leaf whose first graph is another operation's: on the default stream and alive, the captured backward pass is refused; on a side stream, or inside
+    the capture itself, it runs."""
+    block = ff.GatedFeedForward(64, 96).to(gpu_device)
+    params = list(block.parameters())
+    x = torch.randn(20, 64, device=gpu_device, requires_grad=True)
+    dy = torch.randn(20, 64, device=gpu_device)
+    want = torch.autograd.grad(block(x), params + [x], dy)
+    side = torch.cuda.Stream(gpu_device)
+    for penalty_of in (params[0], params[1], x):
+        penalty = penalty_of.square().sum()                            # alive, on the default stream
+        assert penalty.requires_grad
+        with pytest.raises(RuntimeError, match="eager graph"):
+            _captured_gradients(block, x, dy, params + [x])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):                                  # a first call of the block on a side stream does not hide it
+            beside = block(x)
+        with pytest.raises(RuntimeError, match="eager graph"):
+            _captured_gradients(block, x, dy, params + [x])
+        del penalty, beside
+        gc.collect()
+    with torch.cuda.stream(side):
+        penalty = (params[0].square().sum(), x.square().sum(), block(x))
+    torch.cuda.synchronize()
+    _replays_equal(*_captured_gradients(block, x, dy, params + [x]), want)
+    del penalty
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        h = x * 1.0
+        got = torch.autograd.grad(ff.linear(h, params[1].t()[:64], residual=x), [x], dy)
+    _replays_equal(graph, got, torch.autograd.grad(ff.linear(x * 1.0, params[1].t()[:64], residual=x), [x], dy))
+
+
+def test_a_gradient_that_is_not_computed_does_not_refuse_a_capture(gpu_device):
+    x = torch.randn(20, 64, device=gpu_device, requires_grad=True)
+    w = torch.randn(32, 64, device=gpu_device, requires_grad=True)
+    dy = torch.randn(20, 32, device=gpu_device)
+    want = torch.autograd.grad(ff.linear(x, w), [x], dy)
+    penalty = w.square().sum()                                         # alive, on the default stream
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ff.linear(x, w), [x], dy)
+    _replays_equal(graph, got, want)
+    assert penalty.requires_grad

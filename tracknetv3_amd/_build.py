@@ -15,6 +15,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(PKG_DIR, "csrc", "tnv3_capi.hip")
 LIB = os.path.join(PKG_DIR, "libtnv3_hip.so")
 DIAG_LIB = os.path.join(PKG_DIR, "libtnv3_diag.so")
+AUTOGRAD_SRC = os.path.join(PKG_DIR, "csrc", "host", "tnv3_autograd.cpp")
+AUTOGRAD_LIB = os.path.join(PKG_DIR, "libtnv3_autograd.so")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 FAMILIES = ("MISC", "CONV", "WINO", "WINO43", "UP2X", "WGRAD", "TRAIN", "LINEAR")
 # -packed-fp32-ops: no v_pk_add / mul / fma_f32 out of ordinary float code -- some of their forms have given wrong results on this hardware
@@ -58,7 +60,7 @@ def _newer_than(target, paths):
 
 
 def is_stale():
-    return _newer_than(LIB, _sources())
+    return _newer_than(LIB, _sources()) or _newer_than(AUTOGRAD_LIB, [AUTOGRAD_SRC])
 
 
 def _dep_files(depfile):
@@ -104,8 +106,27 @@ def _link(hipcc, objs, lib, verbose):
     os.replace(lib + ".tmp", lib)
 
 
+def _build_autograd(force, verbose):
+    """libtnv3_autograd.so: host code against the installed torch's headers and libraries."""
+    if not force and not _newer_than(AUTOGRAD_LIB, [AUTOGRAD_SRC, __file__]):
+        return
+    import sysconfig
+
+    from torch.utils import cpp_extension
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler: cannot build libtnv3_autograd.so")
+    cmd = [cxx, "-O1", "-std=c++17", "-fPIC", "-shared", "-w"]
+    cmd += [f"-I{d}" for d in cpp_extension.include_paths() + [sysconfig.get_paths()["include"]]] + [AUTOGRAD_SRC]
+    cmd += [f"-L{d}" for d in cpp_extension.library_paths()] + ["-ltorch_python", "-ltorch_cpu", "-lc10", "-o", AUTOGRAD_LIB + ".tmp"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(AUTOGRAD_LIB + ".tmp", AUTOGRAD_LIB)
+
+
 def build(force=False, verbose=False):
-    """Compile every HIP kernel + the C ABI for gfx950.  Cross-compiles without a GPU."""
+    """Compile every HIP kernel + the C ABI for gfx950, and the host library.  Cross-compiles without a GPU."""
     if not force and not is_stale():
         return LIB
     hipcc = _hipcc()
@@ -114,8 +135,10 @@ def build(force=False, verbose=False):
         for f in os.listdir(OBJ_DIR):
             if f.startswith("tnv3_") and not f.startswith("tnv3_diag"):
                 os.remove(os.path.join(OBJ_DIR, f))
-    with ThreadPoolExecutor(max_workers=min(len(FAMILIES), os.cpu_count() or 1)) as pool:
+    with ThreadPoolExecutor(max_workers=min(len(FAMILIES) + 1, os.cpu_count() or 1)) as pool:
+        host = pool.submit(_build_autograd, force, verbose)
         res = list(pool.map(lambda fam: _compile(hipcc, fam, [f"TNV3_TU_{fam}"], verbose), FAMILIES))
+        host.result()
     _link(hipcc, [o for o, _ in res], LIB, verbose)
     return LIB
 

@@ -15,6 +15,7 @@ _c = ctypes
 _f32p = _c.c_void_p
 _lib = None
 _is_emulator = False
+_autograd = None          # libtnv3_autograd.so, loaded when a backward pass is first captured
 ABI_VERSION = 8
 
 
@@ -190,6 +191,26 @@ def load():
         raise Tnv3Error("libtnv3_hip.so ABI version mismatch")
     _lib, _is_emulator = lib, False
     return lib
+
+
+def gradient_streams(ctx):
+    """Stream ids of the nodes that take the gradients which the running backward pass wants from the Function whose context this is (0: the default
+    stream, -1: none, on the CPU)."""
+    global _autograd
+    if _autograd is None:
+        if not os.path.exists(_build.AUTOGRAD_LIB):
+            _build.build()
+        try:
+            lib = _c.PyDLL(_build.AUTOGRAD_LIB)
+        except OSError as e:
+            raise Tnv3Error(f"cannot load {_build.AUTOGRAD_LIB} (built for another torch?): {e}") from e
+        lib.tnv3_gradient_streams.argtypes = [_c.py_object, _c.POINTER(_c.c_longlong), _c.c_int]
+        _autograd = lib
+    out = (_c.c_longlong * 16)()
+    n = _autograd.tnv3_gradient_streams(ctx, out, 16)
+    if not 0 <= n <= 16:
+        raise Tnv3Error(f"tnv3_gradient_streams: {n}")
+    return list(out[:n])
 
 
 def use_library(path):

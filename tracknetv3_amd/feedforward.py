@@ -9,8 +9,9 @@ fp32, bf16 or fp16.  `x` is (..., k) with any leading shape, one position per ro
     y = block(x)                                  # x + W_out (silu(W_gate x) * W_up x)
 
 The pre-activation is kept for the backward pass -- linear's in the tensors' type, gated_linear's in fp32 -- and sums are fp32.
-A captured backward pass needs that no eager graph over the same parameters from the default stream is alive (it is refused otherwise): drop the
-outputs of earlier steps, or run them on a side stream.
+A captured backward pass needs that no eager graph from the default stream, of these layers or of any other operation, is alive over the tensors whose
+gradients it computes: drop the outputs of earlier steps, or run them on a side stream.  For the tensors that these layers are called with it is refused
+otherwise; a tensor that only other operations see is theirs to check.
 """
 import math
 
@@ -45,23 +46,18 @@ def _no_second_derivative():
         raise RuntimeError("linear / gated_linear have no second derivative: backward with create_graph=True is refused")
 
 
-# A leaf's gradient accumulator belongs to the stream on which the first graph over the leaf was recorded and lives as long as any graph over it.  If
-# that is the default stream, a backward pass captured on another would have to make the default stream wait inside the capture, which the runtime
-# answers by ending the process: such a call is refused, before anything of the backward pass is launched.
-def _record_stream_of_accumulators(ctx, x):
-    if x.is_cuda:
-        stream = torch._C._cuda_getCurrentRawStream(x.get_device())
-        for node, _ in ctx.next_functions:
-            if node is not None:
-                node.metadata.setdefault("tnv3_stream", stream)
-
-
+# A leaf's gradient accumulator belongs to the stream on which the first graph over the leaf was recorded, by whatever operation, and lives as long as any
+# graph over it.  If that is the default stream, a backward pass captured on another would have to make the default stream wait inside the capture, which
+# the runtime answers by ending the process: such a call is refused, before anything of the backward pass is launched.
 def _capturable(ctx, x):
     if x.is_cuda and torch._C._cuda_isCurrentStreamCapturing():
-        for node, _ in ctx.next_functions:
-            if node is not None and node.metadata.get("tnv3_stream") == 0:
-                raise RuntimeError("linear / gated_linear: this backward pass is being captured while an eager graph of the same tensors, recorded on the "
-                                   "default stream, is alive: drop its outputs first, or run it on a side stream")
+        _refuse_default_stream(ops._lib.gradient_streams(ctx))
+
+
+def _refuse_default_stream(streams):
+    if 0 in streams:
+        raise RuntimeError("linear / gated_linear: this backward pass is being captured while an eager graph of the same tensors, recorded on the "
+                           "default stream, is alive: drop its outputs first, or run it on a side stream")
 
 
 def _linear_grads(ctx, dy):
@@ -92,7 +88,6 @@ class _Linear(torch.autograd.Function):
         y, pre = ops.linear(x, weight, bias, residual, act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
-        _record_stream_of_accumulators(ctx, x)
         return y
 
     backward = staticmethod(_linear_grads)
@@ -104,7 +99,6 @@ class _GatedLinear(torch.autograd.Function):
         h, pre = ops.gated_linear(x, weight, bias, act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
-        _record_stream_of_accumulators(ctx, x)
         return h
 
     backward = staticmethod(_gated_linear_grads)
