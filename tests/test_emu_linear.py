@@ -355,3 +355,16 @@ def test_which_captured_backward_passes_are_refused(streams, refused):
         return ff._refuse_default_stream(streams)
     with pytest.raises(RuntimeError, match="eager graph"):
         ff._refuse_default_stream(streams)
+
+
+def test_refusals_of_the_modules(emu):
+    for make, text in ((lambda: ff.GatedFeedForward(8, 0), "widths must be positive"), (lambda: ff.GatedFeedForward(0, 8), "widths must be positive"),
+                       (lambda: ff.GatedFeedForward(8, -1), "widths must be positive"), (lambda: ff.Linear(8, 0), "widths must be positive"),
+                       (lambda: ff.Linear(0, 8), "widths must be positive"), (lambda: ff.GatedFeedForward(8, 4, act=9), "unknown activation"),
+                       (lambda: ff.Linear(8, 4, act=None), "unknown activation"), (lambda: ff.Linear(8, 4, act=-1), "unknown activation"),
+                       (lambda: ff.GatedFeedForward(8, 4)(torch.tensor(1.0)), "expects")):
+        with pytest.raises(ValueError, match=text):
+            make()
+    with torch.autocast("cpu", torch.bfloat16), pytest.raises(_lib.Tnv3Error, match="must be torch.bfloat16"):
+        ff.Linear(8, 4)(torch.zeros(2, 8, dtype=torch.bfloat16))
+    assert ff.Linear(8, 4, act=ops.ACT_GELU).act == ops.ACT_GELU

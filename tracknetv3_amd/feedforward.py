@@ -8,7 +8,8 @@ fp32, bf16 or fp16.  `x` is (..., k) with any leading shape, one position per ro
     block = GatedFeedForward(256, 704).to("cuda", torch.bfloat16)
     y = block(x)                                  # x + W_out (silu(W_gate x) * W_up x)
 
-The pre-activation is kept for the backward pass -- linear's in the tensors' type, gated_linear's in fp32 -- and sums are fp32.
+The pre-activation is kept for the backward pass -- linear's in the tensors' type, gated_linear's in fp32 -- and sums are fp32.  All tensors of a call have
+one type: under torch.autocast nothing is cast, a 16-bit input with fp32 weights is refused.  A backward pass with create_graph=True is refused.
 A captured backward pass needs that no eager graph from the default stream, of these layers or of any other operation, is alive over the tensors whose
 gradients it computes: drop the outputs of earlier steps, or run them on a side stream.  For the tensors that these layers are called with it is refused
 otherwise; a tensor that only other operations see is theirs to check.
@@ -26,10 +27,10 @@ ACTIVATIONS = {"none": ops.ACT_NONE, "leaky_relu": ops.ACT_LEAKY_RELU, "sigmoid"
 
 
 def _act(act):
-    if isinstance(act, str):
-        if act not in ACTIVATIONS:
-            raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
+    if isinstance(act, str) and act in ACTIVATIONS:
         return ACTIVATIONS[act]
+    if not isinstance(act, int) or not ops.ACT_NONE <= act <= ops.ACT_GELU_TANH:
+        raise ValueError(f"unknown activation {act!r}: one of {', '.join(ACTIVATIONS)}")
     return act
 
 
@@ -136,6 +137,8 @@ class Linear(nn.Linear):
     """nn.Linear (same parameters and state_dict) with an activation and a residual in the product's epilogue."""
 
     def __init__(self, in_features, out_features, bias=True, act="none", device=None, dtype=None):
+        if in_features < 1 or out_features < 1:
+            raise ValueError(f"Linear: widths must be positive, got {in_features} -> {out_features}")
         super().__init__(in_features, out_features, bias=bias, device=device, dtype=dtype)
         _act(act)
         self.act = act
@@ -150,6 +153,8 @@ class GatedFeedForward(nn.Module):
     def __init__(self, dim, hidden, act="silu", bias=False, residual=True, device=None, dtype=None):
         super().__init__()
         _act(act)
+        if int(dim) < 1 or int(hidden) < 1:
+            raise ValueError(f"GatedFeedForward: widths must be positive, got dim {dim}, hidden {hidden}")
         kw = {"device": device, "dtype": dtype}
         self.dim, self.hidden, self.act, self.residual = int(dim), int(hidden), act, bool(residual)
         self.weight = nn.Parameter(torch.empty(2 * self.hidden, self.dim, **kw))
@@ -161,7 +166,7 @@ class GatedFeedForward(nn.Module):
                 nn.init.uniform_(p, -1 / math.sqrt(fan_in), 1 / math.sqrt(fan_in))      # nn.Linear's range
 
     def forward(self, x):
-        if x.shape[-1] != self.dim:
+        if x.dim() < 1 or x.shape[-1] != self.dim:
             raise ValueError(f"GatedFeedForward expects (..., {self.dim}), got {tuple(x.shape)}")
         h = gated_linear(x, self.weight, self.bias, self.act)
         return linear(h, self.weight_out, self.bias_out, x if self.residual else None)
