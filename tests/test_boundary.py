@@ -126,3 +126,20 @@ def test_infer_split_gate_is_thread_local_and_restored():
         t.start()
         t.join()
     assert not M._NO_SPLIT.active and seen == [False]
+
+
+def test_an_older_build_of_the_same_version_is_refused_by_name(tmp_path, monkeypatch):
+    """Entries were added without a new ABI number: a library that lacks some is named at load time, not at the first call."""
+    import subprocess
+    from tracknetv3_amd import _build, _lib
+    src, lib = tmp_path / "old.c", tmp_path / "libold.so"
+    for body, text in (("int tnv3_abi_version(void) { return 8; }", "older build.*tnv3_linear_forward"),
+                       ("int tnv3_abi_version(void) { return 7; }", "version mismatch"), ("int other(void) { return 0; }", "version mismatch")):
+        src.write_text(body)
+        subprocess.run(["gcc", "-shared", "-fPIC", str(src), "-o", str(lib)], check=True)
+        os.replace(lib, tmp_path / f"lib{len(text)}{len(body)}.so")                # a name of its own: a loaded library is not loaded again
+        monkeypatch.setattr(_build, "LIB", str(tmp_path / f"lib{len(text)}{len(body)}.so"))
+        _lib.reset_library()
+        with pytest.raises(_lib.Tnv3Error, match=text):
+            _lib.load()
+    _lib.reset_library()

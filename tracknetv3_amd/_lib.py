@@ -186,11 +186,19 @@ def load():
         lib = _c.CDLL(path)
     except OSError as e:
         raise Tnv3Error(f"cannot load {path}: {e}") from e
+    _check_library(lib, path)
     _declare(lib)
-    if lib.tnv3_abi_version() != ABI_VERSION:
-        raise Tnv3Error("libtnv3_hip.so ABI version mismatch")
     _lib, _is_emulator = lib, False
     return lib
+
+
+def _check_library(lib, path):
+    """The library is of this version and has every entry: an ABI version only grows by entries, so an older build of the same version may lack some."""
+    missing = [name for name in EXPORTS if not hasattr(lib, name)]
+    if "tnv3_abi_version" in missing or lib.tnv3_abi_version() != ABI_VERSION:
+        raise Tnv3Error(f"{path}: ABI version mismatch")
+    if missing:
+        raise Tnv3Error(f"{path} is an older build: it lacks {', '.join(missing)}; build it again")
 
 
 def gradient_streams(ctx):
