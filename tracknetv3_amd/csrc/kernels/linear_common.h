@@ -24,7 +24,6 @@ typedef unsigned lin_u4_any __attribute__((ext_vector_type(4), aligned(2)));
 typedef float lin_f4_any __attribute__((ext_vector_type(4), aligned(4)));
 
 template <bool V> struct LinFlag { static constexpr bool value = V; };
-template <int V> struct LinCount { static constexpr int value = V; };
 
 struct LinBf16 { unsigned short v; };
 struct LinF16 { unsigned short v; };
@@ -100,8 +99,6 @@ __device__ __forceinline__ float lin_up(float f) { return f; }
 __device__ __forceinline__ void lin_down(float f, LinBf16& o) { o.v = (unsigned short)lin_pack2(f, f, LinBf16{}); }
 __device__ __forceinline__ void lin_down(float f, LinF16& o) { o.v = (unsigned short)lin_pack2(f, f, LinF16{}); }
 __device__ __forceinline__ void lin_down(float f, float& o) { o = f; }
-// the fp32 value that an element of type T keeps of f
-template <class T> __device__ __forceinline__ float lin_round(float f) { T t; lin_down(f, t); return lin_up(t); }
 
 // A pre-activation as a backward pass takes it: rounded to T, but no positive value to 0 -- in fp16 those below 2^-25 would be, and ReLU's derivative at 0
 // is another one.
@@ -324,8 +321,9 @@ __device__ __forceinline__ bool lin_tile(const LinGemmArgs& p, int b, int& ti, i
   return true;
 }
 
-// ---- write-out of eight consecutive columns of one row; v: fp32 sums (gated: v gate, u the other factor)
-template <class T>
+// ---- write-out of eight consecutive columns of one row; v: fp32 sums (gated: v gate, u the other factor).  PLAIN: no pre-activation is
+// kept (a backward pass; known at compile time, its fp16 kernel of 256 x 256 spilled otherwise).
+template <class T, bool PLAIN = false>
 __device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j, float (&v)[8], const float (&bias)[8]) {
   if (i >= p.rows_i || j >= p.rows_j) return;
   const int n = p.rows_j - j < 8 ? (int)(p.rows_j - j) : 8;
@@ -333,7 +331,7 @@ __device__ __forceinline__ void lin_finish8(const LinGemmArgs& p, long i, long j
   const long o = i * p.rows_j + j;
 #pragma unroll
   for (int e = 0; e < 8; ++e) v[e] += bias[e];
-  if (p.pre) lin_store_pre8<T>(static_cast<T*>(p.pre) + o, v, vec, n);
+  if (!PLAIN && p.pre) lin_store_pre8<T>(static_cast<T*>(p.pre) + o, v, vec, n);
   lin_act8<sizeof(T) == 2>(v, p.act);
   if (p.res) {
     float r[8];
@@ -435,7 +433,7 @@ __device__ __forceinline__ void lin_write_out(const LinGemmArgs& p, Put put, flo
           } else if (GATED) {
             lin_finish_gated8<T>(p, i, j, v, u, b0, b1);
           } else {
-            lin_finish8<T>(p, i, j, v, b0);
+            lin_finish8<T, PLAIN>(p, i, j, v, b0);
           }
         }
       }
