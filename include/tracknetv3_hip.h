@@ -569,12 +569,13 @@ int tnv3_absdiff_sum_u8(const unsigned char* frames, const uint16_t* median_x2, 
  * act: 0 none, 1 leaky ReLU (0.01), 2 sigmoid, 3 ReLU, 4 SiLU (z sigmoid z), 5 GELU (z Phi(z)), 6 GELU in its tanh form.
  *   linear   z = x w^T + bias, y = act(z) + residual       x (rows, k), w (n, k), bias (n) or NULL, residual (rows, n) or NULL, y (rows, n)
  *   gated    [g | u] = x w^T + bias, h = act(g) * u        w (2 n, k): the gate's n rows, then the other factor's; bias (2 n) or NULL, h (rows, n)
- * pre (may be NULL): the pre-activation z that the backward call takes: linear (rows, n) in the call's type (act 0 needs none; a
- * positive value stays positive in fp16), gated (rows, 2 n) in
- * fp32 whatever the type.  Tensors are contiguous and start on a 16-byte boundary; widths are free (16-bit ones that are no multiple of 8 cost a
- * copy of the operand, beyond a few rows -- 16 to 64, by size -- and in the backward pass).  1 <= rows <= 2^30, 1 <= widths (2 n for gated) <= 2^20.  An output must
- * not overlap an input.  fp32 products beyond those few rows, and every backward product, run as three bf16 planes per element: fp32's accuracy
- * for elements down to about 2^-110 in size, an absolute 2^-134 below.  Same inputs, same bits.  The workspace (16-byte aligned, at least the queried
+ * pre (may be NULL): the pre-activation z that the backward call takes: linear (rows, n) in the call's type (act 0 needs none; a positive value
+ * stays positive in fp16), gated (rows, 2 n) in fp32 whatever the type.  Tensors are contiguous and start on a 16-byte boundary; widths are free
+ * (16-bit ones that are no multiple of 8 cost a copy of the operand, beyond a few rows -- 16 to 64, by size -- and in the backward pass).
+ * 1 <= rows <= 2^30, 1 <= widths (2 n for gated) <= 2^20; a call one of whose launches would count 2^32 work-items or more is refused (a copy of
+ * 2^35 elements and more).  An output must not overlap an input.  fp32 products beyond those few rows, and every backward product, run as three bf16
+ * planes per element: fp32's accuracy for elements down to about 2^-110 in size, an absolute 2^-134 below.  Same inputs, same bits.  Derivatives are
+ * taken at the pre-activation as it is kept.  The workspace (16-byte aligned, at least the queried
  * size; the query may be 0) is scratch for the one call. */
 size_t tnv3_linear_forward_workspace_bytes(long rows, int k, int n, int dtype);
 int tnv3_linear_forward(const void* x, const void* w, const void* bias, const void* residual, void* y, void* pre, void* workspace,

@@ -5,7 +5,7 @@
 // One barrier per step, placed before the LAST quarter of a step's products: at that point every wave has the step's last fragments in
 // registers and its share of the next stage has landed, so behind the barrier the stage just read can be refilled (a whole step for the loads to
 // arrive) and the next step's first fragments are read under the last quarter's products.  No product waits for a read that was not issued a
-// quarter step (16, 8 or 4 MFMAs of 16 cycles per wave, two waves per SIMD) earlier.
+// quarter step (16, 8 or 4 MFMAs of 16 cycles per wave; two waves per SIMD with two stages, one with four) earlier.
 #pragma once
 #include "linear_common.h"
 

@@ -1,9 +1,11 @@
 // linear_grad.h -- the element-wise part of the position-wise layers' backward passes.
 //   linear  dz = dy act'(z)                                       gated  dz = [dh u act'(g) | dh act(g)],  z = [g | u]
 // The gated layer's z is kept in fp32: rounded to 16 bits, its two factors' errors enter both halves of dz and double the gradients' distance from the
-// exact ones behind a chain of layers (measured: 3.4e-3 of the weight gradient's norm in bf16, a single rounding being 1.7e-3).  dz is rounded to the
-// type, once: it is an operand of both products on the matrix pipe, and a second plane for what the rounding drops would double them (1570 of the
-// 1720 us of a training step of an 8192 x 2048 -> 2 x 5504 -> 2048 block).
+// exact ones behind a chain of layers (measured: 3.4e-3 of the weight gradient's norm in bf16, a single rounding being 1.7e-3).  The linear layer's z is
+// kept in the type: it enters through act' alone and takes the weight gradient from 2.35e-3 to 2.41e-3 off (bf16, any of the smooth activations, dz's and
+// the result's rounding included), where fp32 would write and read 2 more bytes per element.  dz is rounded to the type, once: it is an operand of both
+// products on the matrix pipe, and a second plane for what the rounding drops would double them (1570 of the 1720 us of a training step of an
+// 8192 x 2048 -> 2 x 5504 -> 2048 block).
 // And the bias gradient, the column sums of dz.  Bound by memory: dy and z are read and dz is written once, in 16-byte pieces.  A workgroup takes 256
 // columns (32 work-items of 8) and every 8th row of its row block per work-item; its column sums are joined through LDS and written as
 // partial sums [row block][columns], which lin_colsum adds in order: no atomics, the same bits from run to run.

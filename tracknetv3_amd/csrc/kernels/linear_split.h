@@ -12,9 +12,10 @@
 // overflows, x1 = x2 = 0 for inf / NaN, and inf / NaN taken out of the cross products.  The result is then what fp32 gives.
 //
 // Layout of a step (32 of the contraction, two fragment halves): the elements pass through registers, because a plane is 11 vector instructions per
-// pair to make.  Those run under the matrix pipe: while the first half's products are issued, the next step's elements are split and stored to
-// the other LDS stage, and each register's load for the step after is issued as soon as it is free.  The barrier lies between the halves: the second
-// half's fragments are in registers by then, the next step's first fragments are read under the second half's products.
+// pair to make.  Those stand between the first half's products: while they are issued, the next step's elements are split and stored to the other LDS stage,
+// and each register's load for the step after is issued as soon as it is free.  (They add their time to the products' all the same: two register sets
+// or a finer interleave changed nothing.)  The barrier lies between the halves: the second half's fragments are in registers by then, the next step's
+// first fragments are read under the second half's products.
 #pragma once
 #include "linear_common.h"
 
