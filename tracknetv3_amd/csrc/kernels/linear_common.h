@@ -103,7 +103,9 @@ __device__ __forceinline__ void lin_down(float f, float& o) { o = f; }
 // A pre-activation as a backward pass takes it: rounded to T, but no positive value to 0 -- in fp16 those below 2^-25 would be, and ReLU's derivative at 0
 // is another one.
 template <class T> __device__ __forceinline__ float lin_keep_positive(float z) { return z; }
-template <> __device__ __forceinline__ float lin_keep_positive<LinF16>(float z) { return z > 0.0f && z < 0x1p-24f ? 0x1p-24f : z; }
+template <> __device__ __forceinline__ float lin_keep_positive<LinF16>(float z) {
+  return __builtin_bit_cast(unsigned, z) - 1u < 0x337fffffu ? 0x1p-24f : z;          // 0 < z < 2^-24, in one comparison of the bits
+}
 
 // ---- eight consecutive elements <-> fp32.  vec: all eight exist; else the first `n` one by one (the rest 0).
 __device__ __forceinline__ void lin_unpack8(lin_u4 q, float (&v)[8], LinBf16) {

@@ -36,7 +36,7 @@ def _act(act):
 
 # There is no forward-mode derivative.  autograd says so where an input requires a gradient; otherwise the call would return an output without a tangent.
 def _no_tangents(what, *tensors):
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{what}: an input carries a forward-mode tangent, and the position-wise layers have no forward-mode derivative")
 
 
@@ -116,7 +116,8 @@ def linear(x, weight, bias=None, residual=None, act="none"):
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
-    _no_tangents("linear", x, weight, bias, residual)
+    if forward_ad._current_level >= 0:
+        _no_tangents("linear", x, weight, bias, residual)
     return ops.linear(x, weight, bias, residual, act)
 
 
@@ -129,7 +130,8 @@ def gated_linear(x, weight, bias=None, act="silu"):
     bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, act)
-    _no_tangents("gated_linear", x, weight, bias)
+    if forward_ad._current_level >= 0:
+        _no_tangents("gated_linear", x, weight, bias)
     return ops.gated_linear(x, weight, bias, act)
 
 

@@ -1162,12 +1162,13 @@ def conv1d_k3_wgrad(src0, dpre, src1=None, src_nlc=False):
 # Small calls are bound by what the host does: the checks below look at each tensor once, and the workspace sizes are looked up.
 ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH = 3, 4, 5, 6
 _LINEAR_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_tracing_state = torch._C._get_tracing_state
 _LINEAR_WORKSPACE = {}          # (entry, device, sizes ..) -> bytes: a pure function of its key
 
 
 def _linear_check(what, x, weight, bias, act, gated):
     """(rows, k, n, dtype code) of a position-wise layer's call after its checks."""
-    if torch._C._get_tracing_state() is not None:          # a trace would hold the outputs' allocations and nothing that fills them
+    if _tracing_state() is not None:                       # a trace would hold the outputs' allocations and nothing that fills them
         raise _lib.Tnv3Error(f"{what}: cannot be recorded by torch.jit.trace")
     code = _LINEAR_DTYPES.get(x.dtype)
     if code is None:
