@@ -368,3 +368,33 @@ def test_refusals_of_the_modules(emu):
     with torch.autocast("cpu", torch.bfloat16), pytest.raises(_lib.Tnv3Error, match="must be torch.bfloat16"):
         ff.Linear(8, 4)(torch.zeros(2, 8, dtype=torch.bfloat16))
     assert ff.Linear(8, 4, act=ops.ACT_GELU).act == ops.ACT_GELU
+
+
+def test_inputs_that_are_not_contiguous(emu):
+    """Strides of every kind: the same results and gradients, which have the inputs' shapes; the layer's edges lead to the caller's own nodes (what a
+    captured backward pass is judged by), not to a copy's."""
+    for gated in (False, True):
+        x, w, b, r, dy = lc.make(6, 10, 8, torch.float32, gated, True, True, 4)
+        want = lc.run(x, w, b, None if gated else r, "silu", gated, dy)
+
+        def strided(t):                       # the same values, every second element of a larger tensor, transposed
+            big = torch.zeros(*(2 * s for s in reversed(t.shape)))
+            v = big[tuple(slice(None, None, 2) for _ in t.shape)]
+            v = v.t() if t.dim() == 2 else v
+            return v.copy_(t).detach()
+        leaves = [strided(t).requires_grad_() for t in ([x, w, b] if gated else [x, w, b, r])]
+        assert not any(t.is_contiguous() for t in leaves)
+        y = ff.gated_linear(*leaves, act="silu") if gated else ff.linear(*leaves, act="silu")
+        assert [node.variable.data_ptr() for node, _ in y.grad_fn.next_functions] == [t.data_ptr() for t in leaves]
+        grads = torch.autograd.grad(y, leaves, strided(dy))
+        assert torch.equal(y, want["y"])
+        for name, g, t in zip(("dx", "dw", "db", "dr"), grads, leaves):
+            assert g.shape == t.shape and torch.equal(g, want[name]), name
+        with torch.no_grad():
+            assert torch.equal(ff.gated_linear(*leaves, act="silu") if gated else ff.linear(*leaves, act="silu"), want["y"])
+    # a copy of the input as it was: changing it afterwards does not reach the backward pass
+    xt = torch.randn(10, 6).t()
+    w = torch.randn(8, 10, requires_grad=True)
+    y, x0 = ff.linear(xt, w), xt.clone()
+    xt.mul_(2)
+    assert torch.allclose(torch.autograd.grad(y.sum(), [w])[0], torch.ones(8, 6) @ x0, atol=1e-5)

@@ -385,3 +385,21 @@ def test_a_gradient_that_is_not_computed_does_not_refuse_a_capture(gpu_device):
         got = torch.autograd.grad(ff.linear(x, w), [x], dy)
     _replays_equal(graph, got, want)
     assert penalty.requires_grad
+
+
+def test_a_leaf_that_is_not_contiguous_is_seen_by_the_refusal(gpu_device):
+    x = torch.randn(20, 64, device=gpu_device)
+    w = torch.randn(64, 32, device=gpu_device).t().requires_grad_()
+    dy = torch.randn(20, 32, device=gpu_device)
+    want = torch.autograd.grad(ff.linear(x, w), [w], dy)
+    penalty = w.square().sum()                                         # alive, on the default stream
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(graph):
+            torch.autograd.grad(ff.linear(x, w), [w], dy)
+    del penalty, graph
+    gc.collect()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ff.linear(x, w), [w], dy)
+    _replays_equal(graph, got, want)

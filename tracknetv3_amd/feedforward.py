@@ -83,10 +83,16 @@ def _gated_linear_grads(ctx, dh):
                                      n2 // 2, ops._LINEAR_DTYPES[x.dtype]) + (None,)
 
 
+def _contiguous(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+# (Copies of tensors that are not contiguous are made inside: the Function's edges lead to the caller's own nodes, which _capturable has to see.)
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act):
-        y, pre = ops.linear(x, weight, bias, residual, act, want_pre=True)
+        x, weight = _contiguous(x), _contiguous(weight)
+        y, pre = ops.linear(x, weight, _contiguous(bias), _contiguous(residual), act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
         return y
@@ -97,7 +103,8 @@ class _Linear(torch.autograd.Function):
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, act):
-        h, pre = ops.gated_linear(x, weight, bias, act, want_pre=True)
+        x, weight = _contiguous(x), _contiguous(weight)
+        h, pre = ops.gated_linear(x, weight, _contiguous(bias), act, want_pre=True)
         ctx.save_for_backward(x, weight, pre)
         ctx.act = act
         return h
@@ -109,30 +116,23 @@ def linear(x, weight, bias=None, residual=None, act="none"):
     """act(x weight^T + bias) + residual; x (..., k), weight (n, k), bias (n,), residual (..., n), all of one type.  act: a name of ACTIVATIONS
     or an ops.ACT_* constant.  Differentiable once in every tensor, by a backward pass (a forward-mode tangent is refused)."""
     act = _act(act)
-    x = x if x.is_contiguous() else x.contiguous()
-    weight = weight if weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    residual = residual if residual is None or residual.is_contiguous() else residual.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad) or
                                     (residual is not None and residual.requires_grad)):
         return _Linear.apply(x, weight, bias, residual, act)
     if forward_ad._current_level >= 0:
         _no_tangents("linear", x, weight, bias, residual)
-    return ops.linear(x, weight, bias, residual, act)
+    return ops.linear(_contiguous(x), _contiguous(weight), _contiguous(bias), _contiguous(residual), act)
 
 
 def gated_linear(x, weight, bias=None, act="silu"):
     """act(g) * u with [g | u] = x weight^T + bias; x (..., k), weight (2 n, k) with the gate's n rows first, bias (2 n,).  Differentiable as
     `linear` is."""
     act = _act(act)
-    x = x if x.is_contiguous() else x.contiguous()
-    weight = weight if weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, act)
     if forward_ad._current_level >= 0:
         _no_tangents("gated_linear", x, weight, bias)
-    return ops.gated_linear(x, weight, bias, act)
+    return ops.gated_linear(_contiguous(x), _contiguous(weight), _contiguous(bias), act)
 
 
 class Linear(nn.Linear):
