@@ -283,7 +283,7 @@ def check_least_positive(rows, k, n, act, device):
 # stages, 2 128 x 128 / fp32 128 x 64, 3 256 x 256 / fp32 256 x 128, contraction in parts?, sizes).  For the emulator's CU count (first column) and the card's 256.
 KERNELS_EMU = [
     (1, True, False, 0, 0, False, (65, 40, 40)), (1, True, False, 0, 1, False, (65, 200, 72)), (1, True, False, 0, 2, False, (65, 40, 72)),
-    (4, True, False, 0, 3, False, (257, 392, 392)), (2, True, True, 0, 0, False, (65, 40, 40)), (1, True, True, 0, 1, False, (65, 200, 40)),
+    (1, True, False, 0, 3, False, (130, 264, 136)), (2, True, True, 0, 0, False, (65, 40, 40)), (1, True, True, 0, 1, False, (65, 200, 40)),
     (1, True, True, 0, 2, False, (65, 40, 40)), (1, True, True, 0, 3, False, (130, 264, 72)),
     (4, True, False, 1, 1, False, (257, 40, 40)), (4, True, False, 1, 2, True, (200, 40, 40)), (4, True, False, 1, 3, False, (130, 264, 136)),
     (4, True, False, 1, 3, True, (130, 136, 392)), (4, True, True, 1, 1, False, (65, 40, 136)), (2, True, True, 1, 2, True, (65, 40, 520)),
@@ -307,9 +307,12 @@ KERNELS_GPU = [(256,) + e for e in (
     (False, True, 1, 2, True, (65, 40, 72)), (False, True, 1, 3, False, (520, 4104, 264)), (False, True, 1, 3, True, (130, 520, 2056)))]
 
 
-def check_kernel(half, gated, rows, k, n, device):
+def check_kernel(half, gated, rows, k, n, device, exact_only=False):
     """One kernel of KERNELS_*: bias, activation, residual and a kept pre-activation in the epilogue; real values against the bounds, integers exactly, and in
     fp32 integers that fill all three planes."""
+    if exact_only:
+        check_exact(rows, k, n, torch.bfloat16 if half else torch.float32, gated, bias=True, residual=not gated, device=device, seed=rows + n)
+        return
     for dtype in ((torch.bfloat16, torch.float16) if half else (torch.float32,)):
         check_close(rows, k, n, dtype, "silu", gated, bias=True, residual=not gated, device=device, seed=rows + k + n)
         check_exact(rows, k, n, dtype, gated, bias=True, residual=not gated, device=device, seed=rows + n)
